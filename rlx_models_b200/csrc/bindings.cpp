@@ -615,6 +615,262 @@ void kv_dequant_pages(const Tensor& k8, const Tensor& v8, const Tensor& block_ta
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+// int8 codes [NB, Hkv, 16, D] and their fp32 scales [NB, Hkv] of one cache layer
+static void check_int8_cache(const char* op, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs) {
+  check_cuda(k, "k_cache");
+  TORCH_CHECK(k.scalar_type() == at::kChar && v.scalar_type() == at::kChar && k.dim() == 4 && k.is_contiguous() &&
+                  v.is_contiguous() && v.sizes() == k.sizes() && k.size(2) == 16 && v.device() == k.device(),
+              "b200.", op, ": int8 caches [NB, Hkv, 16, D], contiguous, on one device");
+  TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, "b200.", op, ": head_dim 64 or 128");
+  for (const Tensor* t : {&ks, &vs})
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == k.size(0) &&
+                    t->size(1) == k.size(1) && t->is_contiguous() && t->device() == k.device(),
+                "b200.", op, ": fp32 scales [NB, Hkv], contiguous, on the caches' device");
+  TORCH_CHECK(k.size(0) * k.size(1) * 16 <= INT32_MAX, "b200.", op, ": cache rows exceed 2^31");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0,
+              "b200.", op, ": caches must be 16-byte aligned");
+}
+
+void kv_store_int8(const Tensor& k, const Tensor& v, const Tensor& slots, Tensor& k_cache, Tensor& v_cache,
+                   Tensor& k_scale, Tensor& v_scale, Tensor& status) {
+  check_int8_cache("kv_store_int8", k_cache, v_cache, k_scale, v_scale);
+  const int64_t T = slots.numel(), Hkv = k_cache.size(1), D = k_cache.size(3);
+  for (const Tensor* t : {&k, &v})
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 3 && t->size(0) == T && t->size(1) == Hkv &&
+                    t->size(2) == D && t->device() == k_cache.device() &&
+                    (T == 0 || (t->stride(2) == 1 && t->stride(0) % 8 == 0 && t->stride(1) % 8 == 0 &&
+                                reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0)),
+                "b200.kv_store_int8: k / v bf16 [T, Hkv, D] on the caches' device, rows contiguous and 16-byte aligned");
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
+                  slots.device() == k_cache.device(),
+              "b200.kv_store_int8: slots int64 [T] on the caches' device");
+  c10::cuda::CUDAGuard g(k_cache.device());
+  b200::KvInt8StoreArgs a{};
+  a.k = static_cast<const __nv_bfloat16*>(k.data_ptr());
+  a.v = static_cast<const __nv_bfloat16*>(v.data_ptr());
+  a.k_stride_t = k.stride(0);
+  a.k_stride_h = k.stride(1);
+  a.v_stride_t = v.stride(0);
+  a.v_stride_h = v.stride(1);
+  a.slots = slots.data_ptr<int64_t>();
+  a.k_cache = k_cache.data_ptr<int8_t>();
+  a.v_cache = v_cache.data_ptr<int8_t>();
+  a.k_scale = k_scale.data_ptr<float>();
+  a.v_scale = v_scale.data_ptr<float>();
+  a.T = T;
+  a.num_blocks = k_cache.size(0);
+  a.Hkv = (int)Hkv;
+  a.status = status.data_ptr<int>();
+  b200::kv_int8_store_launch(a, (int)D, cur_stream(k_cache));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+static void check_int8_tables(const char* op, const Tensor& k_cache, const Tensor& tables, const Tensor& ctx) {
+  TORCH_CHECK(tables.scalar_type() == at::kInt && tables.dim() == 2 && tables.is_contiguous() &&
+                  ctx.scalar_type() == at::kInt && ctx.dim() == 1 && ctx.is_contiguous() &&
+                  ctx.numel() == tables.size(0) && tables.device() == k_cache.device() &&
+                  ctx.device() == k_cache.device(),
+              "b200.", op, ": int32 block_tables [B, max_blocks] and ctx_lens [B] on the caches' device");
+  TORCH_CHECK(tables.size(1) < (1 << 27), "b200.", op, ": block_tables too wide");
+}
+
+void kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
+                           const Tensor& block_tables, const Tensor& ctx_lens, Tensor& k_out, Tensor& v_out,
+                           Tensor& status) {
+  check_int8_cache("kv_dequant_pages_int8", k_cache, v_cache, k_scale, v_scale);
+  check_int8_tables("kv_dequant_pages_int8", k_cache, block_tables, ctx_lens);
+  const int64_t B = block_tables.size(0), mb = block_tables.size(1);
+  TORCH_CHECK(B * mb <= INT32_MAX, "b200.kv_dequant_pages_int8: block_tables too large");
+  for (const Tensor* t : {&k_out, &v_out})
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->is_contiguous() && t->dim() == 4 && t->size(0) >= B * mb &&
+                    t->size(1) == k_cache.size(1) && t->size(2) == 16 && t->size(3) == k_cache.size(3) &&
+                    t->device() == k_cache.device(),
+                "b200.kv_dequant_pages_int8: bf16 outputs [>= B * max_blocks, Hkv, 16, D]");
+  c10::cuda::CUDAGuard g(k_cache.device());
+  b200::KvInt8DequantArgs a{};
+  a.k_cache = k_cache.data_ptr<int8_t>();
+  a.v_cache = v_cache.data_ptr<int8_t>();
+  a.k_scale = k_scale.data_ptr<float>();
+  a.v_scale = v_scale.data_ptr<float>();
+  a.tables = block_tables.data_ptr<int32_t>();
+  a.ctx_lens = ctx_lens.data_ptr<int32_t>();
+  a.k_out = static_cast<__nv_bfloat16*>(k_out.data_ptr());
+  a.v_out = static_cast<__nv_bfloat16*>(v_out.data_ptr());
+  a.num_blocks = k_cache.size(0);
+  a.B = (int)B;
+  a.max_blocks = (int)mb;
+  a.Hkv = (int)k_cache.size(1);
+  a.D = (int)k_cache.size(3);
+  a.status = status.data_ptr<int>();
+  b200::kv_int8_dequant_launch(a, cur_stream(k_cache));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// Decode and short multi-token attention over int8 pages; returns the number of launches.
+int64_t paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
+                             const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
+                             const optional<Tensor>& cu_q, int64_t max_q_len, double scale,
+                             const optional<Tensor>& sinks, int64_t window, double softcap, Tensor& out,
+                             Tensor& status) {
+  check_int8_cache("paged_attention_int8", k_cache, v_cache, k_scale, v_scale);
+  check_int8_tables("paged_attention_int8", k_cache, block_tables, ctx_lens);
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.is_contiguous() &&
+                  q.size(2) == k_cache.size(3) && q.device() == k_cache.device(),
+              "b200.paged_attention_int8: q bf16 [T, Hq, D], contiguous, on the caches' device");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.sizes() == q.sizes() &&
+                  out.device() == q.device(),
+              "b200.paged_attention_int8: out like q");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) % 16 == 0,
+              "b200.paged_attention_int8: q and out must be 16-byte aligned");
+  const int64_t T = q.size(0), Hq = q.size(1), Hkv = k_cache.size(1), B = block_tables.size(0);
+  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16, "b200.paged_attention_int8: 1 to 16 query heads per KV head");
+  TORCH_CHECK(B <= 4096, "b200.paged_attention_int8: at most 4096 sequences");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX, "b200.paged_attention_int8: window >= 0");
+  const bool ragged = cu_q.has_value() && cu_q->defined();
+  if (ragged) {
+    TORCH_CHECK(cu_q->scalar_type() == at::kInt && cu_q->numel() == B + 1 && cu_q->is_contiguous() &&
+                    cu_q->device() == q.device() && max_q_len >= 0 && max_q_len * (Hq / Hkv) <= 65535,
+                "b200.paged_attention_int8: cu_q int32 [B + 1] and at most 65535 query rows per KV head");
+  } else {
+    TORCH_CHECK(T == B && max_q_len == 1, "b200.paged_attention_int8: one query per sequence without cu_q");
+  }
+  if (sinks.has_value() && sinks->defined())
+    TORCH_CHECK(sinks->scalar_type() == at::kFloat && sinks->numel() == Hq && sinks->is_contiguous() &&
+                    sinks->device() == q.device(),
+                "b200.paged_attention_int8: sinks f32 [Hq]");
+  if (B == 0 || T == 0 || max_q_len == 0) return 0;
+  c10::cuda::CUDAGuard g(q.device());
+  b200::PagedInt8Args a{};
+  a.q = static_cast<const __nv_bfloat16*>(q.data_ptr());
+  a.k_cache = k_cache.data_ptr<int8_t>();
+  a.v_cache = v_cache.data_ptr<int8_t>();
+  a.k_scale = k_scale.data_ptr<float>();
+  a.v_scale = v_scale.data_ptr<float>();
+  a.tables = block_tables.data_ptr<int32_t>();
+  a.ctx_lens = ctx_lens.data_ptr<int32_t>();
+  a.cu_q = ragged ? cu_q->data_ptr<int32_t>() : nullptr;
+  a.out = static_cast<__nv_bfloat16*>(out.data_ptr());
+  a.sinks = (sinks.has_value() && sinks->defined()) ? sinks->data_ptr<float>() : nullptr;
+  a.num_blocks = k_cache.size(0);
+  a.B = (int)B;
+  a.T = (int)T;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.G = (int)(Hq / Hkv);
+  a.D = (int)q.size(2);
+  a.max_blocks = (int)block_tables.size(1);
+  a.max_q_len = (int)max_q_len;
+  a.window = (int)window;
+  a.scale = (float)scale;
+  a.softcap = (float)softcap;
+  a.status = status.data_ptr<int>();
+  a.device = q.get_device();
+  // a workspace of this call: the allocator orders its reuse by stream, and a captured graph keeps its own
+  Tensor ws = at::empty({b200::paged_int8_ws_floats(a.device, a.B, a.Hkv, a.G, a.D, a.max_q_len, a.max_blocks)},
+                        q.options().dtype(at::kFloat));
+  a.ws = ws.data_ptr<float>();
+  b200::paged_int8_launch(a, cur_stream(q));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return 2;
+}
+
+void kv_copy_blocks(const std::vector<Tensor>& src, const std::vector<Tensor>& dst, const Tensor& src_ids,
+                    const Tensor& dst_ids, Tensor& status) {
+  TORCH_CHECK(!src.empty() && src.size() <= 4 && dst.size() == src.size(),
+              "b200.kv_copy_blocks: one to four tensors and as many destinations");
+  check_cuda(src[0], "src");
+  const auto dev = src[0].device();
+  for (const Tensor* t : {&src_ids, &dst_ids})
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous() && t->device() == dev &&
+                    t->numel() == src_ids.numel(),
+                "b200.kv_copy_blocks: int32 block ids [n] on the caches' device");
+  b200::KvCopyArgs a{};
+  a.parts = (int)src.size();
+  a.layers = (int)src[0].size(0);
+  a.src_blocks = src[0].dim() > 1 ? src[0].size(1) : 0;
+  a.dst_blocks = dst[0].dim() > 1 ? dst[0].size(1) : 0;
+  for (size_t i = 0; i < src.size(); ++i) {
+    const Tensor &s = src[i], &d = dst[i];
+    TORCH_CHECK(s.dim() >= 2 && d.dim() == s.dim() && s.is_contiguous() && d.is_contiguous() &&
+                    s.scalar_type() == d.scalar_type() && s.device() == dev && d.device() == dev,
+                "b200.kv_copy_blocks: contiguous tensors [layers, blocks, ...] of one type on one device");
+    TORCH_CHECK(s.size(0) == a.layers && d.size(0) == a.layers && s.size(1) == a.src_blocks &&
+                    d.size(1) == a.dst_blocks && s.sizes().slice(2) == d.sizes().slice(2),
+                "b200.kv_copy_blocks: layers, blocks and block shapes must match");
+    int64_t bytes = s.element_size();
+    for (int64_t k = 2; k < s.dim(); ++k) bytes *= s.size(k);
+    auto& p = a.part[i];
+    p.src = static_cast<const uint8_t*>(s.data_ptr());
+    p.dst = static_cast<uint8_t*>(d.data_ptr());
+    p.bytes = bytes;
+    p.src_layer = bytes * a.src_blocks;
+    p.dst_layer = bytes * a.dst_blocks;
+  }
+  c10::cuda::CUDAGuard g(dev);
+  a.src_ids = src_ids.data_ptr<int32_t>();
+  a.dst_ids = dst_ids.data_ptr<int32_t>();
+  a.n = src_ids.numel();
+  a.status = status.data_ptr<int>();
+  b200::kv_copy_blocks_launch(a, cur_stream(src[0]));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void verify_drafts(const Tensor& logits, const Tensor& cu_rows, const Tensor& drafts, const optional<Tensor>& probs,
+                   const Tensor& temperature, const Tensor& uniforms, Tensor& tokens, Tensor& accepted) {
+  check_cuda(logits, "logits");
+  const auto dev = logits.device();
+  TORCH_CHECK(logits.scalar_type() == at::kFloat && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+              "b200.verify_drafts: logits f32 [R, V], rows contiguous");
+  const int64_t R = logits.size(0), V = logits.size(1), B = temperature.numel();
+  TORCH_CHECK(V >= 1 && V <= (1 << 24) && R <= 65535, "b200.verify_drafts: 1 to 2^24 tokens, at most 65535 rows");
+  TORCH_CHECK(cu_rows.scalar_type() == at::kInt && cu_rows.numel() == B + 1 && cu_rows.is_contiguous() &&
+                  cu_rows.device() == dev,
+              "b200.verify_drafts: cu_rows int32 [B + 1]");
+  TORCH_CHECK(drafts.scalar_type() == at::kInt && drafts.dim() == 1 && drafts.is_contiguous() &&
+                  drafts.numel() == R - B && drafts.device() == dev,
+              "b200.verify_drafts: drafts int32 [R - B] (every sequence has one row more than drafts)");
+  TORCH_CHECK(temperature.scalar_type() == at::kFloat && temperature.is_contiguous() && temperature.device() == dev &&
+                  uniforms.scalar_type() == at::kFloat && uniforms.numel() == R && uniforms.is_contiguous() &&
+                  uniforms.device() == dev,
+              "b200.verify_drafts: temperature f32 [B], uniforms f32 [R]");
+  TORCH_CHECK(tokens.scalar_type() == at::kInt && tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) >= 1 &&
+                  tokens.is_contiguous() && tokens.device() == dev && accepted.scalar_type() == at::kInt &&
+                  accepted.numel() == B && accepted.is_contiguous() && accepted.device() == dev,
+              "b200.verify_drafts: tokens int32 [B, max_drafts + 1], accepted int32 [B]");
+  const bool has_q = probs.has_value() && probs->defined();
+  if (has_q)
+    TORCH_CHECK(probs->scalar_type() == at::kFloat && probs->dim() == 2 && probs->size(0) == R - B &&
+                    probs->size(1) == V && (V <= 1 || probs->stride(1) == 1) && probs->device() == dev,
+                "b200.verify_drafts: draft_probs f32 [R - B, V], rows contiguous");
+  if (B == 0) return;
+  c10::cuda::CUDAGuard g(dev);
+  b200::VerifyArgs a{};
+  a.logits = logits.data_ptr<float>();
+  a.ld = logits.stride(0);
+  a.cu_rows = cu_rows.data_ptr<int32_t>();
+  a.drafts = drafts.data_ptr<int32_t>();
+  a.probs = has_q ? probs->data_ptr<float>() : nullptr;
+  a.ldp = has_q ? probs->stride(0) : 0;
+  a.temperature = temperature.data_ptr<float>();
+  a.uniforms = uniforms.data_ptr<float>();
+  a.tokens = tokens.data_ptr<int32_t>();
+  a.accepted = accepted.data_ptr<int32_t>();
+  a.R = R;
+  a.ND = R - B;
+  a.B = (int)B;
+  a.V = (int)V;
+  a.max_drafts = (int)tokens.size(1) - 1;
+  a.chunks = b200::verify_chunks(a.V);
+  // sums of 8 bytes, maxima and indexes of 4: one workspace of this call
+  const int64_t n = R * a.chunks;
+  Tensor ws = at::empty({2 * n}, logits.options().dtype(at::kDouble));
+  a.part_sum = ws.data_ptr<double>();
+  a.part_max = reinterpret_cast<float*>(a.part_sum + n);
+  a.part_arg = reinterpret_cast<int32_t*>(a.part_max + n);
+  b200::verify_drafts_launch(a, cur_stream(logits));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
 void argmax(const Tensor& logits, Tensor& out) {
   check_cuda(logits, "logits");
   TORCH_CHECK(logits.scalar_type() == at::kFloat && logits.dim() == 2 && logits.stride(1) == 1, "b200.argmax");
@@ -1651,6 +1907,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("scale_by", &scale_by);
   m.def("instance_norm", &instance_norm);
   m.def("kv_dequant_pages", &kv_dequant_pages);
+  m.def("kv_store_int8", &kv_store_int8);
+  m.def("kv_dequant_pages_int8", &kv_dequant_pages_int8);
+  m.def("paged_attention_int8", &paged_attention_int8);
+  m.def("kv_copy_blocks", &kv_copy_blocks);
+  m.def("verify_drafts", &verify_drafts);
   m.def("act_im2col", &act_im2col);
   m.def("lstm_cell", &lstm_cell);
   m.def("convt_fold", &convt_fold);

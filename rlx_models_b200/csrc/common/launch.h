@@ -333,6 +333,79 @@ void prefill_attention_launch(const AttnArgs& a, cudaStream_t st);
 bool fmha_supported(const AttnArgs& a);
 void fmha_launch(const AttnArgs& a, cudaStream_t st);
 
+// Paged KV cache in 8 bits: int8 codes [NB, Hkv, 16, D] with one power-of-two fp32 scale per
+// (block, KV head) [NB, Hkv]: see attention/kv_int8.cu.
+struct KvInt8StoreArgs {
+  const __nv_bfloat16* k;  // [T, Hkv, D] with the strides below (elements, multiples of 8)
+  const __nv_bfloat16* v;
+  int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const int64_t* slots;    // [T] block * 16 + offset (< 0: skip); tokens of one block are adjacent
+  int8_t* k_cache;
+  int8_t* v_cache;
+  float* k_scale;
+  float* v_scale;
+  int64_t T, num_blocks;
+  int Hkv;
+  int group = 1;           // tokens per warp (set by the launcher)
+  int* status;
+};
+void kv_int8_store_launch(const KvInt8StoreArgs& a, int D, cudaStream_t st);
+
+// bf16 copies of the pages of a prefill batch at block b * max_blocks + p (as kv_dequant_pages_launch)
+struct KvInt8DequantArgs {
+  const int8_t* k_cache;
+  const int8_t* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* tables;    // [B, max_blocks]
+  const int32_t* ctx_lens;  // [B]
+  __nv_bfloat16* k_out;
+  __nv_bfloat16* v_out;
+  int64_t num_blocks;
+  int B, max_blocks, Hkv, D;
+  int* status;
+};
+void kv_int8_dequant_launch(const KvInt8DequantArgs& a, cudaStream_t st);
+
+struct PagedInt8Args {
+  const __nv_bfloat16* q;  // [T, Hq, D]
+  const int8_t* k_cache;
+  const int8_t* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* tables;    // [B, max_blocks]
+  const int32_t* ctx_lens;  // [B] keys of each sequence, its new tokens included
+  const int32_t* cu_q;      // [B + 1] query offsets, or null: one query per sequence
+  __nv_bfloat16* out;       // [T, Hq, D]
+  const float* sinks;       // [Hq] or null
+  float* ws;                // paged_int8_ws_floats() floats
+  int64_t num_blocks;
+  int B, T, Hq, Hkv, G, D, max_blocks, max_q_len, window;
+  float scale, softcap;
+  int* status;
+  int device;
+};
+int64_t paged_int8_ws_floats(int device, int B, int Hkv, int G, int D, int max_q_len, int max_blocks);
+void paged_int8_launch(const PagedInt8Args& a, cudaStream_t st);
+
+// Blocks of a cache copied over all layers, up to four tensors in one launch: see attention/kv_copy.cu.
+struct KvCopyArgs {
+  struct Part {
+    const uint8_t* src;
+    uint8_t* dst;
+    int64_t src_layer, dst_layer;  // bytes between layers
+    int64_t bytes;                 // bytes of one block in one layer
+    int pieces;                    // CTAs per block (set by the launcher; 0: copied with the first piece)
+  } part[4];
+  int parts;
+  const int32_t* src_ids;  // [n], < 0: skip
+  const int32_t* dst_ids;  // [n]
+  int64_t n, src_blocks, dst_blocks;
+  int layers;
+  int* status;
+};
+void kv_copy_blocks_launch(const KvCopyArgs& a, cudaStream_t st);
+
 // Attention backward for training (causal, dense [T, H, D] rows, head_dim 128):
 // see train/attn_bwd.cu.
 struct AttnBwdArgs {
@@ -528,6 +601,27 @@ struct SampleArgs {
   int64_t ws_elems;
 };
 void sample_launch(const SampleArgs& a, cudaStream_t st);
+
+// Speculative sampling: accept drafted tokens, draw the next one: see sampling/verify.cu.
+struct VerifyArgs {
+  const float* logits;      // [R, V], row stride ld
+  int64_t ld;
+  const int32_t* cu_rows;   // [B + 1] rows of each sequence: its drafts' and one more
+  const int32_t* drafts;    // [R - B]
+  const float* probs;       // [R - B, V] (row stride ldp) the drafter's probabilities, or null: certain drafts
+  int64_t ldp;
+  const float* temperature; // [B]
+  const float* uniforms;    // [R] in [0, 1)
+  int32_t* tokens;          // [B, max_drafts + 1]
+  int32_t* accepted;        // [B]
+  int64_t R, ND;
+  int B, V, max_drafts, chunks;
+  float* part_max;          // [R, chunks]
+  double* part_sum;         // [R, chunks]
+  int32_t* part_arg;        // [R, chunks]
+};
+int verify_chunks(int V);
+void verify_drafts_launch(const VerifyArgs& a, cudaStream_t st);
 // repetition / frequency / presence penalties + logit bias, in place (CSR per row)
 void penalties_launch(float* logits, int64_t ld, int64_t B, int64_t V, const int32_t* off, const int32_t* ids,
                       const int32_t* counts, const float* rep, const float* freq, const float* pres,

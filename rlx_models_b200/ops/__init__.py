@@ -15,7 +15,8 @@ from ._ext import count_launches as _count
 
 __all__ = [
     "linear", "linear_swiglu", "rmsnorm", "qkv_rope", "embedding", "decode_attention",
-    "prefill_attention", "argmax", "sample", "interleave_gate_up", "rope_inv_freq",
+    "prefill_attention", "kv_store_int8", "kv_dequant_pages_int8", "paged_attention_int8", "kv_copy_blocks",
+    "verify_drafts", "argmax", "sample", "interleave_gate_up", "rope_inv_freq",
     "check_errors", "KernelError", "available",
 ]
 
@@ -315,6 +316,139 @@ def prefill_attention(q, k_cache, v_cache, block_tables, ctx_lens, cu_q, max_q_l
     ext().prefill_attention(q, k_cache, v_cache, block_tables, ctx_lens, cu_q, out, sinks, int(window),
                             float(scale), int(max_q_len), s.status, bool(causal), bool(q_paged), float(softcap))
     return out
+
+
+def kv_store_int8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                  v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """Quantise new rows into an int8 paged cache, in place.
+
+    k / v bf16 [T, Hkv, D] (D 64 or 128; row views with 16-byte aligned strides
+    are read as they are), slots int64 [T] = block * 16 + offset, negative =
+    skip; caches int8 [NB, Hkv, 16, D], scales fp32 [NB, Hkv]. Per (block, head):
+    s = 2^e, the smallest e >= -100 with max|x| <= 127 s; code = rint(x / s). A
+    block written at offset 0 starts over (offsets not written hold 0); any other
+    write keeps its rows and s' = max(s_old, s), the old codes becoming
+    rint(code * s_old / s'). NaN is stored as 0 and +-inf as +-127 s, neither
+    counts in the maximum.
+
+    The tokens of one block must be adjacent in the batch; a slot that comes
+    twice among them takes the later row."""
+    if k.stride(-1) != 1 or (k.stride(0) | k.stride(1)) % 8 or k.data_ptr() % 16:
+        k = k.contiguous()
+    if v.stride(-1) != 1 or (v.stride(0) | v.stride(1)) % 8 or v.data_ptr() % 16:
+        v = v.contiguous()
+    _count(1)
+    ext().kv_store_int8(k, v, slots, k_cache, v_cache, k_scale, v_scale, scratch(k_cache.device).status)
+
+
+def kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens):
+    """bf16 copies (exact) of the int8 pages a batch reads: page p of sequence b
+    goes to block b * max_blocks + p of the returned [B * max_blocks, Hkv, 16, D]
+    caches, whose block table is returned with them. Pages at or past
+    ceil(ctx_lens[b] / 16) stay uninitialised (the first one of an empty
+    sequence is zero)."""
+    B, mb = block_tables.shape
+    shape = (B * mb,) + tuple(k_cache.shape[1:])
+    kb = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
+    vb = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
+    _count(1)
+    ext().kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, kb, vb,
+                                scratch(k_cache.device).status)
+    return kb, vb, torch.arange(B * mb, dtype=torch.int32, device=k_cache.device).view(B, mb)
+
+
+INT8_DIRECT_ROWS = 64  # query rows per KV head up to which attention reads the int8 pages directly
+
+
+def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, block_tables: torch.Tensor, ctx_lens: torch.Tensor, *,
+                         cu_q: torch.Tensor | None = None, max_q_len: int = 1, scale: float,
+                         sinks: torch.Tensor | None = None, window: int = 0, softcap: float = 0.0,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over int8 pages (see ``kv_store_int8``), grouped heads.
+
+    q bf16 [T, Hq, D], D 64 or 128, up to 16 query heads per KV head. Without
+    ``cu_q`` every sequence has one query (decode, T = B); with ``cu_q`` int32
+    [B + 1] sequence b has the queries cu_q[b] .. cu_q[b + 1] (at most
+    ``max_q_len``), the last of its ``ctx_lens[b]`` tokens. ``sinks`` fp32 [Hq],
+    ``window`` (0 = all) and ``softcap`` as in ``decode_attention``. A query that
+    sees no key gives 0; rows of ``out`` behind cu_q[B] are left as they are.
+
+    Up to ``INT8_DIRECT_ROWS`` query rows per KV head the pages are read as they
+    are; longer chunks are bound by their products and go through bf16 copies of
+    the pages to ``prefill_attention``, whose tcgen05 products outweigh the
+    copies (unless its tiles do not take the group size)."""
+    if out is None:
+        out = torch.empty_like(q)
+    Hq, Hkv = q.shape[1], k_cache.shape[1]
+    if (cu_q is not None and max_q_len * Hq > INT8_DIRECT_ROWS * Hkv and 128 * Hkv % Hq == 0
+            and block_tables.shape[1] > 0):
+        kb, vb, tables = kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens)
+        return prefill_attention(q, kb, vb, tables, ctx_lens, cu_q, max_q_len, scale=scale, sinks=sinks,
+                                 window=window, out=out, softcap=softcap)
+    _count(ext().paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q,
+                                      int(max_q_len), float(scale), sinks, int(window), float(softcap), out,
+                                      scratch(q.device).status))
+    return out
+
+
+def _block_ids(ids, device) -> torch.Tensor:
+    if torch.is_tensor(ids):
+        return ids
+    return torch.tensor(list(ids), dtype=torch.int32).to(device, non_blocking=True)
+
+
+def kv_copy_blocks(src, dst, src_ids, dst_ids) -> None:
+    """``dst[i][:, dst_ids] = src[i][:, src_ids]`` for up to four tensors
+    [layers, blocks, ...] of a cache (K, V, scales), all layers in one launch.
+    ``src`` and ``dst`` may be the same tensors. Block ids: int32 tensors [n] on
+    the device (negative: skip), or lists, which are checked here. A block may be
+    copied to several places; the places must differ, and none may be a source
+    of the same call (copies run in no order)."""
+    if not torch.is_tensor(src_ids) and not torch.is_tensor(dst_ids):
+        src_ids, dst_ids = [int(i) for i in src_ids], [int(i) for i in dst_ids]
+        ns, nd = src[0].shape[1], dst[0].shape[1]
+        if len(src_ids) != len(dst_ids):
+            raise ValueError("kv_copy_blocks: as many destinations as sources")
+        if any(not 0 <= i < ns for i in src_ids) or any(not 0 <= i < nd for i in dst_ids):
+            raise ValueError("kv_copy_blocks: block id out of range")
+        if len(set(dst_ids)) != len(dst_ids):
+            raise ValueError("kv_copy_blocks: a destination block comes twice")
+        if src[0].data_ptr() == dst[0].data_ptr() and set(src_ids) & set(dst_ids):
+            raise ValueError("kv_copy_blocks: a destination block is also a source")
+    dev = src[0].device
+    _count(1)
+    ext().kv_copy_blocks(list(src), list(dst), _block_ids(src_ids, dev), _block_ids(dst_ids, dev),
+                         scratch(dev).status)
+
+
+def verify_drafts(logits: torch.Tensor, cu_rows: torch.Tensor, drafts: torch.Tensor,
+                  draft_probs: torch.Tensor | None, temperature: torch.Tensor, uniforms: torch.Tensor, *,
+                  max_drafts: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Speculative sampling: accept drafted tokens against the target's
+    probabilities and draw the token behind them.
+
+    Sequence b owns the rows cu_rows[b] .. cu_rows[b + 1] of ``logits`` fp32
+    [R, V]: one for each of its drafts and one more (at least one); ``drafts``
+    int32 [R - B] and ``draft_probs`` fp32 [R - B, V] follow in the same order
+    (None: the drafts were certain, e.g. greedy or looked up). With
+    p = softmax(logits / temperature[b]) and u = ``uniforms`` fp32 [R] in [0, 1),
+    draft i is accepted while u[row i] * q(draft) < p(draft). At the first
+    refusal the next token is drawn from max(p - q, 0), after the last
+    acceptance from p of the row behind it: the first token whose running sum
+    exceeds u[last row of b] times the total. temperature <= 0: accepted while it
+    is the lowest argmax, then the argmax. Logits of -inf and NaN have
+    probability 0; a row without a finite logit refuses its draft and gives 0.
+
+    Returns tokens int32 [B, max_drafts + 1] (accepted drafts, the new token,
+    then -1) and the number of accepted drafts int32 [B]. All decisions are made
+    in 64 bits."""
+    B = temperature.numel()
+    tokens = torch.empty(B, int(max_drafts) + 1, dtype=torch.int32, device=logits.device)
+    accepted = torch.empty(B, dtype=torch.int32, device=logits.device)
+    _count(2)
+    ext().verify_drafts(logits, cu_rows, drafts, draft_probs, temperature, uniforms, tokens, accepted)
+    return tokens, accepted
 
 
 def argmax(logits: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -156,3 +156,94 @@ def instance_norm(x: torch.Tensor, gamma=None, beta=None, active: int = 0, eps: 
     if beta is not None:
         y = y + beta.float()[None, :, None]
     return y
+
+
+def pow2_scale(amax: float) -> float:
+    """Smallest 2^e, e >= -100, with amax <= 127 * 2^e."""
+    e = -100
+    while amax > 127.0 * 2.0 ** e:
+        e += 1
+    return 2.0 ** e
+
+
+def store_int8(x: torch.Tensor, slots: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> None:
+    """One of K / V of ``ops.kv_store_int8``, in place and in 64 bits: x [T, Hkv, D]
+    rows into codes int8 [NB, Hkv, 16, D], scale fp32 [NB, Hkv]. Blocks in the order
+    of their first token; within a block the last row of a slot counts."""
+    blocks: dict[int, dict[int, int]] = {}
+    for t, s in enumerate(slots.tolist()):
+        if s >= 0:
+            blocks.setdefault(s // 16, {})[s % 16] = t
+    for b, rows in blocks.items():
+        off, tok = list(rows.keys()), list(rows.values())
+        v = x[tok].double()  # [n, Hkv, D]
+        fin = torch.where(torch.isfinite(v), v, torch.zeros_like(v)).abs().amax((0, 2))
+        for h in range(x.shape[1]):
+            s = pow2_scale(float(fin[h]))
+            old = codes[b, h].double()
+            if 0 in rows:
+                old = torch.zeros_like(old)
+            else:
+                prev = float(scale[b, h])
+                s = max(s, prev)
+                old = torch.round(old * (prev / s))
+            old[off] = torch.round(torch.nan_to_num(v[:, h] / s, nan=0.0, posinf=127.0, neginf=-127.0))
+            codes[b, h] = old.to(torch.int8)
+            scale[b, h] = s
+
+
+def verify_drafts(logits: torch.Tensor, cu_rows: list[int], drafts: list[int], draft_probs, temperature: list[float],
+                  uniforms: list[float], max_drafts: int):
+    """``ops.verify_drafts`` in 64 bits, one sequence after the other: (tokens, accepted)."""
+    V, out, acc = logits.shape[1], [], []
+
+    def dist(row, t):
+        x = logits[row].double()
+        x = torch.where(torch.isnan(x), torch.full_like(x, -float("inf")), x).clamp(max=3.4028234663852886e38)
+        top = x.max()
+        if torch.isinf(top):
+            return None, 0
+        first = int((x == top).nonzero()[0])
+        return (torch.softmax((x - top) / t, 0) if t > 0 else None), first
+
+    for b, t in enumerate(temperature):
+        r0, r1 = cu_rows[b], cu_rows[b + 1]
+        n, got = min(r1 - r0 - 1, max_drafts), []
+        new = None
+        for i in range(n):
+            d = drafts[r0 - b + i]
+            p, first = dist(r0 + i, t)
+            q = None if draft_probs is None else torch.nan_to_num(draft_probs[r0 - b + i].double()).clamp(min=0)
+            if not t > 0:
+                ok = p is None and d == first and torch.isfinite(logits[r0 + i]).any()
+                w = None
+            elif p is None:
+                ok, w = False, None
+            else:
+                qd = 1.0 if q is None else (float(q[d]) if 0 <= d < V else 0.0)
+                ok = 0 <= d < V and uniforms[r0 + i] * qd < float(p[d])
+                if q is None:
+                    w = p.clone()
+                    if 0 <= d < V:
+                        w[d] = 0.0
+                else:
+                    w = (p - q).clamp(min=0)
+                if float(w.sum()) == 0.0:
+                    w = p
+            if not ok:
+                new = (w, first)
+                break
+            got.append(d)
+        if new is None:
+            p, first = dist(r0 + n, t)
+            new = (p if t > 0 else None, first)
+        w, first = new
+        if w is None:
+            tok = first
+        else:
+            c = w.cumsum(0)
+            hit = (c > uniforms[r1 - 1] * float(c[-1])).nonzero()
+            tok = int(hit[0]) if hit.numel() else int((w > 0).nonzero()[-1])
+        acc.append(len(got))
+        out.append(got + [tok] + [-1] * (max_drafts - len(got)))
+    return out, acc
