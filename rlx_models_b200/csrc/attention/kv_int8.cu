@@ -222,27 +222,32 @@ __global__ void __launch_bounds__(256) dequant_kernel(KvInt8DequantArgs a) {
 // ---------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------
-// Work is cut evenly over the grid, whatever the lengths: the pages of every
-// (sequence, KV head, block of query rows) lie end to end in one line of units,
-// CTA i takes units [i U / N, (i + 1) U / N). A segment that one CTA covers is
-// written out by it, the parts of the others are joined by merge_kernel, which
-// repeats the same arithmetic; so the workspace has two slots per CTA and does
-// not grow with the contexts.
+// Work is cut evenly over the warps of the grid, whatever the lengths: the pages
+// of every (sequence, KV head, block of query rows) lie end to end in one line of
+// units, warp i takes units [i c, (i + 1) c). A segment that one warp covers is
+// written out by it, the parts of the others are joined by merge_kernel; so the
+// workspace has two slots per warp (the segment it begins inside, the one it ends
+// inside) and does not grow with the contexts. Warps do not meet: no barrier
+// stands in the way of the loads, and the ring of a warp runs on into its next
+// segment (block ids, then pages, are asked for while the last one is worked on).
 //
-// Inside a CTA the four warps take pages in turn, each with its own TMA ring
-// (no exchange between warps until a segment ends), running maximum, sum and
-// accumulators. Both products run transposed, S^T = K Q^T and O^T = V^T P^T
-// (mma m16n8k16, f16 operands, f32 sums): the 16 keys of a page and 16 of its
-// columns fill the 16-row operand, and 8 query rows (the group of a KV head) the
-// 8-column one, half the multiplies of the other orientation for a group of 4.
+// Each warp has its own TMA ring, running maximum, sum and accumulators. Both
+// products run transposed, S^T = K Q^T and O^T = V^T P^T (mma m16n8k16, f16
+// operands, f32 sums): the 16 keys of a page and 16 of its columns fill the 16-row
+// operand, and 8 query rows (the group of a KV head) the 8-column one, half the
+// multiplies of the other orientation for a group of 4.
 //   * K: ldmatrix hands a thread 4 consecutive codes of a key; a product does
 //     not care in which order its terms come, so Q is held in that order.
 //   * V: ldmatrix.trans moves pairs of bytes, a thread gets (d, d + 1) of two
 //     keys: rows g and g + 8 of the operand are columns 2 g and 2 g + 1.
-//   * codes widen exactly: the byte code + 128 under the exponent of 1024 is
-//     1024 + 128 + code in f16; K subtracts 1152 and folds its scale into the
-//     scores, V computes code * (s / s_ref) by one fma, with s_ref the largest
-//     V scale of the warp's pages so far (powers of two: exact down to 2^-24).
+//   * codes become f16 without arithmetic: the byte code + 128 in the low bits of
+//     a half is the subnormal (code + 128) 2^-24, which the tensor cores multiply
+//     exactly; 3 integer instructions for 4 codes, where converting costs 5 (the
+//     loop is bound by instruction issue, not by HBM). The offset is taken out
+//     exactly: S starts at -128 sum(q), and O gets one more product per tile with
+//     the constant -128 (page by page, so that nothing accumulates to cancel).
+//     2^24 and the block's K scale go into the factor of the scores, its V scale
+//     relative to the largest so far, s / s_ref, into the weights.
 //   * Q is scaled by a power of two per row to below 2, so that any bf16 row
 //     keeps its 8 bits in f16. P is rounded to f16 (2^-12 of each weight).
 //   * weights are 2^(score - m) with m 8 below the running maximum, so that f16
@@ -254,18 +259,17 @@ template <int D_, int NT_>
 struct Cfg {
   static constexpr int D = D_, NT = NT_, ROWS = 8 * NT_, STEPS = D_ / 16;
   static constexpr int PAGE = 16 * D_, STAGE = 2 * PAGE;
-  static constexpr int CTAS = NT_ == 1 ? 4 : (NT_ == 2 ? 3 : 2);  // resident per SM (registers)
-  static constexpr int NST = (NT_ <= 2 ? 3 : (NT_ == 3 ? 4 : 5)) * (D_ == 64 ? 2 : 1);
+  static constexpr int PP = NT_ == 1 ? 2 : 1;    // pages a warp works on at once
+  static constexpr int CTAS = 2;                 // resident per SM (registers)
+    // Pages on their way per warp. Deeper rings are slower: 3 pages of 4 KB for each of 8 warps of an SM already fill
+  // the memory system, and what is asked for beyond only delays block ids, scales and queries behind it (64 requests
+  // of 512 to 2304 tokens, 12 warps an SM: 52.6 us with 4 pages, 47.6 with 3, 45.2 with 2; 8 warps with 3: 45.2).
+  static constexpr int NST = 3 * (D_ == 64 ? 2 : 1);
   static constexpr int RING = 4 * NST * STAGE;
-  static constexpr int OLD = D_ + 4;  // padded row of the exchange buffer, in floats
-  static constexpr int EXCH = 4 * ROWS * OLD * 4;
-  static constexpr int MAIN = RING > EXCH ? RING : EXCH;
   static constexpr int QLD = D_ * 2 + 32;  // padded Q row in bytes (conflict-free 8-byte loads)
-  static constexpr bool QS = NT_ > 2;      // Q in shared memory instead of registers
-  static constexpr int QBYTES = QS ? ROWS * QLD : 0;
-  static constexpr int STATS = 4 * ROWS * 3 * 4;
-  static constexpr int FIXED = MAIN + QBYTES + STATS + 4 * NST * 8 + 64;
-  static constexpr int smem(int B) { return 1024 + FIXED + (B + 1) * 8; }
+  static constexpr int QBYTES = ROWS * QLD;  // per warp
+  static constexpr int FIXED = RING + 4 * QBYTES + 4 * NST * 8 + 16;
+  static constexpr int smem(int B) { return 1024 + FIXED + (B + 1) * 4; }
 };
 
 struct SeqInfo {
@@ -291,13 +295,8 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedInt8Args& a, int b) {
   return s;
 }
 
-__device__ __forceinline__ int64_t cta_begin(int64_t i, int64_t U, int64_t N) { return i * U / N; }
-
-// CTAs that work when there are U units: at least 4 units (one per warp) each.
-__device__ __forceinline__ int64_t active_ctas(int64_t U, int grid) {
-  const int64_t n = (U + 3) / 4;
-  return n < grid ? n : grid;
-}
+// Units per warp: at least 4, below which joining parts costs more than the pages.
+__device__ __forceinline__ int warp_units(int U, int grid) { return max(4, (U + 4 * grid - 1) / (4 * grid)); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -319,24 +318,20 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-__device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
-  const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
-  const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
-                            *reinterpret_cast<__half2*>(&c));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   const __half2 r = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t dup_h2(float a) { return pack_h2(a, a); }
+// 4 codes -> (code + 128) 2^-24 as f16 subnormals, two to a register: `flip` first, then bytes 0 and 2, bytes 1 and 3.
+__device__ __forceinline__ uint32_t flip(uint32_t w) { return w ^ 0x80808080u; }
+__device__ __forceinline__ uint32_t codes_even(uint32_t u) { return __byte_perm(u, 0, 0x4240); }
+__device__ __forceinline__ uint32_t codes_odd(uint32_t u) { return __byte_perm(u, 0, 0x4341); }
+constexpr uint32_t kMinus128 = 0x80808080u;  // f16x2 of -128 * 2^-24
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kShift = 8.f;  // m: the running maximum minus this (log2), see above
 constexpr float kLimit = 15.f;  // a score above m + kLimit moves m
+constexpr float kNone = -1e30f; // m before the first visible key: finite, so that a masked score (-inf) has weight 0
 
 // Byte offset of 16-byte chunk c of row r in a page written by TMA with the
 // swizzle of its row width (128-byte rows: chunk ^ row; 64-byte rows: chunk ^ row / 2).
@@ -350,27 +345,20 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
                                                                      const __grid_constant__ CUtensorMap tmV,
                                                                      PagedInt8Args a) {
   using C = Cfg<D, NT>;
-  constexpr int ROWS = C::ROWS, STEPS = C::STEPS, NST = C::NST;
+  constexpr int ROWS = C::ROWS, STEPS = C::STEPS, NST = C::NST, PP = C::PP;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t* qs = base + C::MAIN;
-  float* st_m = reinterpret_cast<float*>(qs + C::QBYTES);  // [4][ROWS] per warp: maximum, sum, V reference scale
-  float* st_l = st_m + 4 * ROWS;
-  float* st_r = st_l + 4 * ROWS;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(st_r + 4 * ROWS);
-  int64_t* wsum = reinterpret_cast<int64_t*>(bars + 4 * NST);  // [4] + failure flag
-  int* s_fail = reinterpret_cast<int*>(wsum + 4);
-  int64_t* pre = reinterpret_cast<int64_t*>(base + C::FIXED);
-
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  uint64_t* full = bars + warp * NST;
   uint8_t* ring = base + warp * NST * C::STAGE;
+  uint8_t* qs = base + C::RING + warp * C::QBYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + C::RING + 4 * C::QBYTES) + warp * NST;
+  int* wsum = reinterpret_cast<int*>(base + C::RING + 4 * C::QBYTES + 4 * NST * 8);
+  int* pre = reinterpret_cast<int*>(base + C::FIXED);  // [B + 1] units in front of each sequence
 
   if (lane == 0)
     for (int i = 0; i < NST; ++i) mbar_init(&full[i], 1);
   if (tid == 0) {
-    *s_fail = 0;
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
@@ -380,43 +368,50 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
 
   // prefix sums of the units of every sequence
   const int per = (a.B + 127) / 128;
-  int64_t mine = 0;
+  int mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
     if (b < a.B) {
       const SeqInfo s = seq_info<ROWS>(a, b);
-      mine += (int64_t)a.Hkv * s.rb * s.pages;
+      mine += a.Hkv * s.rb * s.pages;
     }
   }
-  int64_t inc = mine;
+  int inc = mine;
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
   if (lane == 31) wsum[warp] = inc;
   __syncthreads();
-  int64_t run = inc - mine;
+  int run = inc - mine;
   for (int w = 0; w < warp; ++w) run += wsum[w];
+  const int U = wsum[0] + wsum[1] + wsum[2] + wsum[3];
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
     if (b < a.B) {
       pre[b] = run;
-      const SeqInfo s = seq_info<ROWS>(a, b);
-      run += (int64_t)a.Hkv * s.rb * s.pages;
+      if (blockIdx.x == 0) a.ws_pre[b] = run;  // for merge_kernel
+      if (i + 1 < per) {
+        const SeqInfo s = seq_info<ROWS>(a, b);
+        run += a.Hkv * s.rb * s.pages;
+      }
     }
   }
-  const int64_t U = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-  if (tid == 0) pre[a.B] = U;
+  if (tid == 0) {
+    pre[a.B] = U;
+    if (blockIdx.x == 0) a.ws_pre[a.B] = U;
+  }
   __syncthreads();
-  const int64_t N = active_ctas(U, gridDim.x);
-  if (blockIdx.x >= N) return;
-  const int64_t u0 = cta_begin(blockIdx.x, U, N), u1 = cta_begin(blockIdx.x + 1, U, N);
+  const int chunk = warp_units(U, gridDim.x);
+  const int worker = blockIdx.x * 4 + warp;
+  if ((int64_t)worker * chunk >= U) return;
+  const int u0 = worker * chunk, u1 = min(u0 + chunk, U);
 
-  const uint32_t bias = 0xE480E480u;  // f16x2 of -1152
-  uint32_t it = 0;                    // pages this warp has taken from its ring (stage and parity)
-  int64_t u = u0;
-  int b = 0;
-  {  // last b with pre[b] <= u0 (empty sequences share a prefix: take the last)
+  // ---- the part of a segment at hand: units [u, ue) of [seg0, seg1), its first page, its rows ----
+  int u = u0, ue, seg0, seg1, page, cnt;
+  int b, h, row0, nrows, pos0, first_pos, last_pos, q0;
+  const int32_t* tab;
+  {  // last b with pre[b] <= u0 (empty sequences share a prefix: the last of them is not empty)
     int lo = 0, hi = a.B;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -425,189 +420,295 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
     }
     b = lo;
   }
-
-  while (u < u1) {
-    while (pre[b + 1] <= u) ++b;
-    const SeqInfo sq = seq_info<ROWS>(a, b);
-    const int64_t rel = u - pre[b];
-    const int hs = (int)(rel / sq.pages);
-    const int h = hs / sq.rb, rb = hs % sq.rb;
-    const int64_t seg0 = pre[b] + (int64_t)hs * sq.pages, seg1 = seg0 + sq.pages;
-    const int64_t ue = seg1 < u1 ? seg1 : u1;
-    const int pa = sq.lo + (int)(u - seg0), pb = sq.lo + (int)(ue - seg0);
-    const int row0 = rb * ROWS, nrows = min(ROWS, sq.n * a.G - row0);
-    const int pos0 = sq.ctx - sq.n;  // position of the first new token
-
-    // ---- pages of this warp: pa + warp + 4 j, j < cnt; lane i holds the block of page j = 32 k + i ----
-    const int cnt = pb - pa > warp ? (pb - pa - warp + 3) / 4 : 0;
-    const int32_t* tab = a.tables + (int64_t)b * a.max_blocks + pa + warp;
-    auto fetch = [&](int j0, int& id, float& sk, float& sv) {
-      id = 0;
-      sk = sv = 0.f;
-      if (j0 + lane < cnt) {
-        id = tab[4 * (j0 + lane)];
-        if (id < 0 || id >= a.num_blocks) {
-          report_error(a.status, kErrBounds, id);
-          id = 0;
-        } else {
-          sk = a.k_scale[(int64_t)id * a.Hkv + h];
-          sv = a.v_scale[(int64_t)id * a.Hkv + h];
-        }
+  // Lane i holds page j = 32 k + i of the current 32 and of the next: its first row in the cache, its scales; and the
+  // block id of the 32 after. They are loaded 16 pages and more before they are needed.
+  int y0 = 0, y1 = 0, id = 0;
+  float sk0 = 0.f, sk1 = 0.f, sv0 = 0.f, sv1 = 0.f;
+  // the part that follows: its first block ids (lane i: page i < n_cnt), its KV head
+  int n_id = 0, n_cnt = 0, n_h = 0;
+  auto load_ids = [&](int j0) { id = j0 + lane < cnt ? tab[j0 + lane] : 0; };
+  auto known = [&](int i) { return i >= 0 && i < a.num_blocks; };
+  auto resolve = [&](int j0, int& y, float& sk, float& sv) {
+    y = 0;
+    sk = sv = 0.f;
+    if (j0 + lane < cnt) {
+      if (known(id)) {
+        const int row = id * a.Hkv + h;
+        y = row * 16;
+        sk = a.k_scale[row];
+        sv = a.v_scale[row];
+      } else {
+        report_error(a.status, kErrBounds, id);
       }
-    };
-    int id0, id1;
-    float sk0, sk1, sv0, sv1;
-    fetch(0, id0, sk0, sv0);
-    auto issue = [&](int id, uint32_t slot) {  // one lane
-      uint8_t* dst = ring + slot * C::STAGE;
-      mbar_arrive_expect_tx(&full[slot], C::STAGE);
-      const int y = (id * a.Hkv + h) * 16;
-      tma_load_2d(dst, &tmK, &full[slot], 0, y);
-      tma_load_2d(dst + C::PAGE, &tmV, &full[slot], 0, y);
-    };
-#pragma unroll 1
-    for (int j = 0; j < NST && j < cnt; ++j) {
-      const int id = __shfl_sync(0xffffffffu, id0, j);
-      if (lane == 0) issue(id, (it + j) % NST);
     }
-    fetch(32, id1, sk1, sv1);
-
-    // ---- Q: rows n = g of each tile in the order of the K fragments, scaled to below 2 ----
-    uint32_t qf[C::QS ? 1 : NT][STEPS][2];
-    float rs[NT][2];  // score factors of columns 2 t4 and 2 t4 + 1
+  };
+  int ui = u0;                                           // next unit to be asked for
+  uint32_t in_slot = 0, out_slot = 0, out_phase = 0;     // ring positions
+  auto issue = [&](int y) {
+    if (lane == 0) {
+      uint8_t* dst = ring + in_slot * C::STAGE;
+      mbar_arrive_expect_tx(&full[in_slot], C::STAGE);
+      tma_load_2d(dst, &tmK, &full[in_slot], 0, y);
+      tma_load_2d(dst + C::PAGE, &tmV, &full[in_slot], 0, y);
+    }
+    in_slot = in_slot + 1 == NST ? 0 : in_slot + 1;
+    ++ui;
+  };
+  auto next_slot = [&]() {
+    if (++out_slot == NST) {
+      out_slot = 0;
+      out_phase ^= 1;
+    }
+  };
+  // (pages, rows and head of the segment that unit v lies in; b moves on to its sequence)
+  auto segment_of = [&](int v, int& bb, SeqInfo& sq, int& hs) {
+    while (pre[bb + 1] <= v) ++bb;
+    sq = seq_info<ROWS>(a, bb);
+    hs = (v - pre[bb]) / sq.pages;
+  };
+  auto locate = [&]() {
+    SeqInfo sq;
+    int hs;
+    segment_of(u, b, sq, hs);
+    h = hs / sq.rb;
+    seg0 = pre[b] + hs * sq.pages;
+    seg1 = seg0 + sq.pages;
+    ue = seg1 < u1 ? seg1 : u1;
+    cnt = ue - u;
+    page = sq.lo + u - seg0;
+    tab = a.tables + (int64_t)b * a.max_blocks + page;
+    row0 = (hs % sq.rb) * ROWS;
+    nrows = min(ROWS, sq.n * a.G - row0);
+    q0 = sq.q0;
+    pos0 = sq.ctx - sq.n;
+    first_pos = pos0 + row0 / a.G;
+    last_pos = pos0 + (row0 + nrows - 1) / a.G;
+  };
+  auto peek = [&]() {  // at the part behind this one
+    n_cnt = 0;
+    if (ue < u1) {
+      int nb = b, hs;
+      SeqInfo sq;
+      segment_of(ue, nb, sq, hs);
+      n_h = hs / sq.rb;
+      n_cnt = min(sq.pages, u1 - ue);
+      n_id = lane < n_cnt ? a.tables[(int64_t)nb * a.max_blocks + sq.lo + lane] : 0;
+    }
+  };
+  // Q: rows n = g of each tile in the order of the K fragments, scaled to below 2. The rows are asked for as soon as
+  // the segment is known (fetch_q) and put in place when they are there (place_q).
+  uint2 qraw[NT][STEPS];
+  float rs[NT][2], s_init[NT][2];  // score factors and starts (-128 sum q) of columns 2 t4 and 2 t4 + 1
+  int posc[NT][2];                 // their positions
+  auto fetch_q = [&]() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + nt * 8 + g;
-      uint2 w[STEPS];
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) qraw[nt][s] = make_uint2(0, 0);
+      if (nt * 8 + g < nrows) {
+        const int r = row0 + nt * 8 + g, tok = r / a.G, head = h * a.G + r % a.G;
+        const __nv_bfloat16* qp = a.q + ((int64_t)(q0 + tok) * a.Hq + head) * D + 4 * t4;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) qraw[nt][s] = *reinterpret_cast<const uint2*>(qp + 16 * s);
+      }
+    }
+  };
+  auto place_q = [&]() {
+    __syncwarp();  // every lane has read the rows of the last segment
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       uint32_t am = 0;
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) w[s] = make_uint2(0, 0);
-      if (nt * 8 + g < nrows) {
-        const int tok = r / a.G, head = h * a.G + r % a.G;
-        const __nv_bfloat16* qp = a.q + ((int64_t)(sq.q0 + tok) * a.Hq + head) * D + 4 * t4;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) w[s] = *reinterpret_cast<const uint2*>(qp + 16 * s);
+      for (int s = 0; s < STEPS; ++s) {
+        const uint2 w = qraw[nt][s];
+        am = max(am, max(max(w.x & 0x7fffu, (w.x >> 16) & 0x7fffu), max(w.y & 0x7fffu, (w.y >> 16) & 0x7fffu)));
       }
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s)
-        am = max(am, max(max(w[s].x & 0x7fffu, (w[s].x >> 16) & 0x7fffu),
-                         max(w[s].y & 0x7fffu, (w[s].y >> 16) & 0x7fffu)));
       am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
-      const int e = min(max((int)(am >> 7) - 127, -100), 120);
+      const int e = min(max((int)(am >> 7) - 127, -100), 100);
       const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23);
+      float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
-        const uint32_t x = pack_h2(bf16_lo(w[s].x) * down, bf16_hi(w[s].x) * down);
-        const uint32_t y = pack_h2(bf16_lo(w[s].y) * down, bf16_hi(w[s].y) * down);
-        if constexpr (C::QS) {
-          if (warp == 0) *reinterpret_cast<uint2*>(qs + (nt * 8 + g) * C::QLD + 32 * s + 8 * t4) = make_uint2(x, y);
-        } else {
-          qf[nt][s][0] = x;
-          qf[nt][s][1] = y;
-        }
+        // codes (0, 2) and (1, 3) of a word meet in one operand register
+        const uint2 w = qraw[nt][s];
+        const uint32_t x = pack_h2(bf16_lo(w.x) * down, bf16_lo(w.y) * down);
+        const uint32_t y = pack_h2(bf16_hi(w.x) * down, bf16_hi(w.y) * down);
+        const float2 fx = __half22float2(*reinterpret_cast<const __half2*>(&x));
+        const float2 fy = __half22float2(*reinterpret_cast<const __half2*>(&y));
+        sum += (fx.x + fx.y) + (fy.x + fy.y);
+        *reinterpret_cast<uint2*>(qs + (nt * 8 + g) * C::QLD + 32 * s + 8 * t4) = make_uint2(x, y);
       }
-      rs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t4) * a.scale;
-      rs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t4 + 4) * a.scale;
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= -128.f / 16777216.f;
+      const float f = up * a.scale * (16777216.f * (a.softcap > 0.f ? 1.f : kLog2e));
+      const int pos = pos0 + (row0 + nt * 8 + g) / a.G;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        rs[nt][c] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4 * c);
+        s_init[nt][c] = __shfl_sync(0xffffffffu, sum, 8 * t4 + 4 * c);
+        posc[nt][c] = __shfl_sync(0xffffffffu, pos, 8 * t4 + 4 * c);
+      }
     }
-    if constexpr (C::QS) __syncthreads();
+    __syncwarp();
+  };
+
+  locate();
+  load_ids(0);
+  fetch_q();
+
+  while (true) {
+    // ids of the first 32 pages are here or on their way; some of the pages may have been asked for already
+    resolve(0, y0, sk0, sv0);
+#pragma unroll 1
+    while (ui < ue && ui < u + NST) issue(__shfl_sync(0xffffffffu, y0, ui - u));
+    load_ids(32);
+    place_q();
+    peek();
 
     float o[NT][STEPS][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = kNone;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) o[nt][s][0] = o[nt][s][1] = o[nt][s][2] = o[nt][s][3] = 0.f;
     }
     float sref = 0.f, iref = 0.f;
-    // positions of this thread's columns (query rows 2 t4, 2 t4 + 1 of each tile)
-    const int first_pos = pos0 + row0 / a.G, last_pos = pos0 + (row0 + max(nrows, 1) - 1) / a.G;
-
-    int j = 0;
-    bool dead = false;
+    int key0 = page * 16;
 #pragma unroll 1
-    for (; j < cnt; ++j) {
-      if ((j & 31) == 0 && j > 0) {
-        id0 = id1;
-        sk0 = sk1;
-        sv0 = sv1;
-        fetch(j + 32, id1, sk1, sv1);
+    for (int j = 0; j < cnt; j += PP, key0 += 16 * PP) {
+      if ((j & 15) == 0) {
+        if ((j & 31) != 0) {
+          resolve(j + 16, y1, sk1, sv1);
+          load_ids(j + 48);
+        } else if (j > 0) {
+          y0 = y1;
+          sk0 = sk1;
+          sv0 = sv1;
+        }
       }
-      const uint32_t n_it = it + j;
-      const uint32_t slot = n_it % NST;
-      const float sk = __shfl_sync(0xffffffffu, sk0, j & 31);
-      const float sv = __shfl_sync(0xffffffffu, sv0, j & 31);
-      const int jn = j + NST;
-      const int idn = __shfl_sync(0xffffffffu, (jn >> 5) == (j >> 5) ? id0 : id1, jn & 31);
-      if (!mbar_wait(&full[slot], (n_it / NST) & 1, a.status, kErrTimeoutFull)) {
-        dead = true;
-        break;
-      }
-      const uint32_t kb = smem_u32(ring + slot * C::STAGE), vb = kb + C::PAGE;
-      // codes of the page into registers, then the slot is free for page j + NST
-      uint32_t kw[STEPS][2], vw[STEPS][2];
+      // codes of the pages into registers, then their slots are free for the pages NST further on
+      uint32_t kw[PP][STEPS][2], vw[PP][STEPS][2];
+      float sk[PP], sv[PP];
 #pragma unroll
-      for (int s = 0; s < STEPS; s += 2) {
-        const uint32_t off = page_off<D>((lane & 7) + ((lane >> 3) & 1) * 8, s + (lane >> 4));
-        ldmatrix_x4(kb + off, kw[s][0], kw[s][1], kw[s + 1][0], kw[s + 1][1]);
-        ldmatrix_x4_trans(vb + off, vw[s][0], vw[s][1], vw[s + 1][0], vw[s + 1][1]);
+      for (int p = 0; p < PP; ++p) {
+        sk[p] = __shfl_sync(0xffffffffu, sk0, j + p);
+        sv[p] = __shfl_sync(0xffffffffu, sv0, j + p);
+        if (p == 0 || j + p < cnt) {
+          if (!mbar_wait(&full[out_slot], out_phase, a.status, kErrTimeoutFull)) {
+            // copies in flight land before the CTA leaves (those behind the one given up on)
+            for (int k = u + j + p + 1; k < ui; ++k) {
+              next_slot();
+              if (!mbar_wait(&full[out_slot], out_phase, a.status, kErrTimeoutDrain)) break;
+            }
+            return;
+          }
+          const uint32_t kb = smem_u32(ring) + out_slot * C::STAGE, vb = kb + C::PAGE;
+          next_slot();
+#pragma unroll
+          for (int s = 0; s < STEPS; s += 2) {
+            const uint32_t off = page_off<D>((lane & 7) + ((lane >> 3) & 1) * 8, s + (lane >> 4));
+            ldmatrix_x4(kb + off, kw[p][s][0], kw[p][s][1], kw[p][s + 1][0], kw[p][s + 1][1]);
+            ldmatrix_x4_trans(vb + off, vw[p][s][0], vw[p][s][1], vw[p][s + 1][0], vw[p][s + 1][1]);
+          }
+        } else {  // an odd last page: the other half is masked below, and its weights are 0 times whatever is here
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) kw[p][s][0] = kw[p][s][1] = vw[p][s][0] = vw[p][s][1] = 0;
+        }
       }
-      __syncwarp();
-      if (lane == 0 && jn < cnt) issue(idn, slot);
-
       // S^T = K Q^T
-      float sc[NT][4];
+      float sc[PP][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const uint32_t x = kw[s][0] ^ 0x80808080u, y = kw[s][1] ^ 0x80808080u;
-        const uint32_t a0 = h2_add(__byte_perm(x, 0x64646464u, 0x4140), bias);
-        const uint32_t a1 = h2_add(__byte_perm(y, 0x64646464u, 0x4140), bias);
-        const uint32_t a2 = h2_add(__byte_perm(x, 0x64646464u, 0x4342), bias);
-        const uint32_t a3 = h2_add(__byte_perm(y, 0x64646464u, 0x4342), bias);
+      for (int p = 0; p < PP; ++p)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          if constexpr (C::QS) {
-            const uint2 q2 = *reinterpret_cast<const uint2*>(qs + (nt * 8 + g) * C::QLD + 32 * s + 8 * t4);
-            mma_f16(sc[nt], a0, a1, a2, a3, q2.x, q2.y);
-          } else {
-            mma_f16(sc[nt], a0, a1, a2, a3, qf[nt][s][0], qf[nt][s][1]);
+          sc[p][nt][0] = sc[p][nt][2] = s_init[nt][0];
+          sc[p][nt][1] = sc[p][nt][3] = s_init[nt][1];
+        }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {
+        uint2 q2[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          q2[nt] = *reinterpret_cast<const uint2*>(qs + (nt * 8 + g) * C::QLD + 32 * s + 8 * t4);
+#pragma unroll
+        for (int p = 0; p < PP; ++p) {
+          const uint32_t x = flip(kw[p][s][0]), y = flip(kw[p][s][1]);
+          const uint32_t a0 = codes_even(x), a1 = codes_even(y), a2 = codes_odd(x), a3 = codes_odd(y);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[p][nt], a0, a1, a2, a3, q2[nt].x, q2[nt].y);
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int p = 0; p < PP; ++p) {
+        const int i = ui - u;  // page of this part, or of the next one
+        if (i < min(j + PP, cnt) + NST) {  // (an odd last page frees one slot only)
+          if (i < cnt) {
+            issue(__shfl_sync(0xffffffffu, (i ^ j) < 32 ? y0 : y1, i));
+          } else if (i - cnt < n_cnt) {
+            const int v = __shfl_sync(0xffffffffu, n_id, i - cnt);
+            issue(known(v) ? (v * a.Hkv + n_h) * 16 : 0);
           }
         }
       }
 
       // scores in units of log2, masks
-      const int key0 = (pa + warp + 4 * j) * 16;
-      const bool edge = key0 + 15 > first_pos || (a.window > 0 && key0 <= last_pos - a.window);
+#pragma unroll
+      for (int p = 0; p < PP; ++p)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f0 = rs[nt][0] * sk[p], f1 = rs[nt][1] * sk[p];
+          sc[p][nt][0] *= f0;
+          sc[p][nt][1] *= f1;
+          sc[p][nt][2] *= f0;
+          sc[p][nt][3] *= f1;
+        }
+      if (a.softcap > 0.f) {
+        const float icap = 1.f / a.softcap, cap = a.softcap * kLog2e;
+#pragma unroll
+        for (int p = 0; p < PP; ++p)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[p][nt][i] = cap * tanhf(sc[p][nt][i] * icap);
+      }
+      const bool edge = key0 + 16 * PP - 1 > first_pos || (a.window > 0 && key0 <= last_pos - a.window) || j + PP > cnt;
+      if (edge) {
+#pragma unroll
+        for (int p = 0; p < PP; ++p)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = key0 + 16 * p + g + (i >> 1) * 8;
+              const int pos = posc[nt][i & 1];
+              if (key > pos || (a.window > 0 && key <= pos - a.window) || j + p >= cnt) sc[p][nt][i] = -INFINITY;
+            }
+      }
       bool grow = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = sc[nt][i] * (rs[nt][i & 1] * sk);
-          if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
-          x *= kLog2e;
-          if (edge) {
-            const int key = key0 + g + (i >> 1) * 8;
-            const int pos = pos0 + (row0 + nt * 8 + 2 * t4 + (i & 1)) / a.G;
-            if (key > pos || (a.window > 0 && key <= pos - a.window)) x = -INFINITY;
-          }
-          sc[nt][i] = x;
-          grow |= x > m[nt][i & 1] + kLimit;
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(sc[0][nt][c], sc[0][nt][2 + c]);
+          if constexpr (PP == 2) mx = fmaxf(mx, fmaxf(sc[PP - 1][nt][c], sc[PP - 1][nt][2 + c]));
+          grow |= mx > m[nt][c] + kLimit;
         }
-      }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(m[nt][c], fmaxf(sc[nt][c], sc[nt][2 + c]) - kShift);
+            float mx = fmaxf(sc[0][nt][c], sc[0][nt][2 + c]);
+            if constexpr (PP == 2) mx = fmaxf(mx, fmaxf(sc[PP - 1][nt][c], sc[PP - 1][nt][2 + c]));
+            mx = fmaxf(m[nt][c], mx - kShift);
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float f = mx == -INFINITY ? 1.f : ex2(m[nt][c] - mx);
+            const float f = ex2(m[nt][c] - mx);
             m[nt][c] = mx;
             l[nt][c] *= f;
 #pragma unroll
@@ -618,195 +719,205 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
           }
         }
       }
-      // weights, transposed to the operand order
-      uint32_t pf[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-        const float p0 = ex2(sc[nt][0] - m0), p1 = ex2(sc[nt][1] - m1);
-        const float p2 = ex2(sc[nt][2] - m0), p3 = ex2(sc[nt][3] - m1);
-        l[nt][0] += p0 + p2;
-        l[nt][1] += p1 + p3;
-        pf[nt][0] = transpose8x8(pack_h2(p0, p1));
-        pf[nt][1] = transpose8x8(pack_h2(p2, p3));
-      }
-      // O^T += V^T P^T
-      if (sv > sref) {  // a larger V scale: the sums are kept in units of the largest
-        const float f = sref / sv;
+      const float sv_max = PP == 2 ? fmaxf(sv[0], sv[PP - 1]) : sv[0];
+      if (sv_max > sref) {  // a larger V scale: the sums are kept in units of the largest
+        const float f = sref / sv_max;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int s = 0; s < STEPS; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[nt][s][i] *= f;
-        sref = sv;
-        iref = 1.f / sv;
+        sref = sv_max;
+        iref = 1.f / sv_max;
       }
-      const float c = sv * iref;
-      const uint32_t c2 = dup_h2(c), n2 = dup_h2(-1152.f * c);
+      // weights, transposed to the operand order
+      uint32_t pf[PP][NT][2];
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        const uint32_t x = vw[s][0] ^ 0x80808080u, y = vw[s][1] ^ 0x80808080u;
-        const uint32_t a0 = h2_fma(__byte_perm(x, 0x64646464u, 0x4240), c2, n2);
-        const uint32_t a1 = h2_fma(__byte_perm(x, 0x64646464u, 0x4341), c2, n2);
-        const uint32_t a2 = h2_fma(__byte_perm(y, 0x64646464u, 0x4240), c2, n2);
-        const uint32_t a3 = h2_fma(__byte_perm(y, 0x64646464u, 0x4341), c2, n2);
+      for (int p = 0; p < PP; ++p) {
+        const float c = sv[p] * iref;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][s], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
-      }
-    }
-    if (dead) {  // copies in flight land before the CTA leaves
-      const int issued = min(cnt, j + NST);
-      for (int k = j + 1; k < issued; ++k)
-        if (!mbar_wait(&full[(it + k) % NST], ((it + k) / NST) & 1, a.status, kErrTimeoutDrain)) break;
-      if (lane == 0) *s_fail = 1;
-    }
-    it += cnt;
-
-    // ---- join the four warps ----
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float s = l[nt][c];
-        s += __shfl_xor_sync(0xffffffffu, s, 4);
-        s += __shfl_xor_sync(0xffffffffu, s, 8);
-        s += __shfl_xor_sync(0xffffffffu, s, 16);
-        if (g == 0) {
-          const int r = nt * 8 + 2 * t4 + c;
-          st_m[warp * ROWS + r] = m[nt][c];
-          st_l[warp * ROWS + r] = s;
-          st_r[warp * ROWS + r] = sref;
+        for (int nt = 0; nt < NT; ++nt) {
+          const float p0 = ex2(sc[p][nt][0] - m[nt][0]), p1 = ex2(sc[p][nt][1] - m[nt][1]);
+          const float p2 = ex2(sc[p][nt][2] - m[nt][0]), p3 = ex2(sc[p][nt][3] - m[nt][1]);
+          l[nt][0] += p0 + p2;
+          l[nt][1] += p1 + p3;
+          pf[p][nt][0] = transpose8x8(pack_h2(p0 * c, p1 * c));
+          pf[p][nt][1] = transpose8x8(pack_h2(p2 * c, p3 * c));
         }
       }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int p = 0; p < PP; ++p)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          const uint32_t x = flip(vw[p][s][0]), y = flip(vw[p][s][1]);
+          const uint32_t a0 = codes_even(x), a1 = codes_odd(x), a2 = codes_even(y), a3 = codes_odd(y);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][s], a0, a1, a2, a3, pf[p][nt][0], pf[p][nt][1]);
+        }
+#pragma unroll
+      for (int p = 0; p < PP; ++p)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            mma_f16(o[nt][s], kMinus128, kMinus128, kMinus128, kMinus128, pf[p][nt][0], pf[p][nt][1]);
     }
-    __syncthreads();  // every ring is drained: its memory becomes the exchange buffer
-    if (*s_fail) return;
-    float* exch = reinterpret_cast<float*>(base);
+
+    // ---- the rows of this part: out, or to the workspace ----
+    const bool whole = seg0 >= u0 && seg1 <= u1;
+    float* part = a.ws + ((int64_t)worker * 2 + (seg0 < u0 ? 0 : 1)) * ROWS * (D + 2);
+    const float unit = sref * 16777216.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        float sum = l[nt][c];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int r = nt * 8 + 2 * t4 + c;
         if (r < nrows) {
-          float* dst = exch + (warp * ROWS + r) * C::OLD + 2 * g;
+          if (whole) {
+            const int rr = row0 + r, head = h * a.G + rr % a.G;
+            float f = unit;
+            if (a.sinks != nullptr) {
+              const float sk2 = a.sinks[head] * kLog2e, top = fmaxf(m[nt][c], sk2), fm = ex2(m[nt][c] - top);
+              sum = sum * fm + ex2(sk2 - top);
+              f *= fm;
+            }
+            f = sum == 0.f ? 0.f : f / sum;  // no visible key: 0
+            __nv_bfloat16* dst = a.out + ((int64_t)(q0 + rr / a.G) * a.Hq + head) * D + 2 * g;
 #pragma unroll
-          for (int s = 0; s < STEPS; ++s)
-            *reinterpret_cast<float2*>(dst + 16 * s) = make_float2(o[nt][s][c], o[nt][s][2 + c]);
+            for (int s = 0; s < STEPS; ++s)
+              *reinterpret_cast<uint32_t*>(dst + 16 * s) = pack_bf16x2(o[nt][s][c] * f, o[nt][s][2 + c] * f);
+          } else {
+            float* dst = part + r * D + 2 * g;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+              *reinterpret_cast<float2*>(dst + 16 * s) = make_float2(o[nt][s][c] * unit, o[nt][s][2 + c] * unit);
+            if (g == 0) {
+              part[ROWS * D + r] = m[nt][c];
+              part[ROWS * D + ROWS + r] = sum;
+            }
+          }
         }
       }
     }
-    __syncthreads();
-    const bool whole = seg0 >= u0 && seg1 <= u1;
-    float* part = a.ws + ((int64_t)blockIdx.x * 2 + (seg0 < u0 ? 0 : 1)) * ROWS * (D + 2);
-    for (int i = tid; i < nrows * (D / 4); i += 128) {
-      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, st_m[w * ROWS + r]);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float mw = st_m[w * ROWS + r];
-        const float f = mw == -INFINITY ? 0.f : ex2(mw - mx), fr = f * st_r[w * ROWS + r];  // (0 * NaN stays NaN)
-        const float4 v = *reinterpret_cast<const float4*>(exch + (w * ROWS + r) * C::OLD + d);
-        sum += f * st_l[w * ROWS + r];
-        acc.x += fr * v.x;
-        acc.y += fr * v.y;
-        acc.z += fr * v.z;
-        acc.w += fr * v.w;
-      }
-      const int rr = row0 + r, tok = rr / a.G, head = h * a.G + rr % a.G;
-      if (whole) {
-        if (a.sinks != nullptr && mx != -INFINITY) {
-          const float sk2 = a.sinks[head] * kLog2e, top = fmaxf(mx, sk2), f = ex2(mx - top);
-          sum = sum * f + ex2(sk2 - top);
-          acc.x *= f;
-          acc.y *= f;
-          acc.z *= f;
-          acc.w *= f;
-        }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no visible key: 0
-        uint2* dst = reinterpret_cast<uint2*>(a.out + ((int64_t)(sq.q0 + tok) * a.Hq + head) * D + d);
-        *dst = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-      } else {
-        *reinterpret_cast<float4*>(part + r * D + d) = acc;
-        if (d == 0) {
-          part[ROWS * D + r] = mx;
-          part[ROWS * D + ROWS + r] = sum;
-        }
-      }
-    }
-    fence_proxy_async_smem();  // the exchange buffer is written by TMA next
-    __syncthreads();
     u = ue;
+    if (u >= u1) break;
+    locate();
+    id = n_id;
+    fetch_q();
   }
 }
 
-// Joins the parts of the segments that several CTAs share and writes zeros for
-// rows without keys. One CTA of D threads per (sequence, query row of a KV head).
+// Joins the parts of the segments that several warps share and writes zeros for
+// rows without keys. D / 4 lanes hold a row; with few rows several such groups
+// share a row's parts (a context that is cut over many CTAs has few rows next to
+// it), with many a CTA takes as many rows as it has groups.
+constexpr int kMergeThreads = 256;
+
 template <int D, int NT>
-__global__ void __launch_bounds__(D) merge_kernel(PagedInt8Args a, int grid) {
-  using C = Cfg<D, NT>;
-  constexpr int ROWS = C::ROWS, NW = D / 32;
-  __shared__ int64_t s_sum[2][NW];
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(PagedInt8Args a, int grid) {
+  constexpr int ROWS = 8 * NT, LANES = D / 4, GROUPS = kMergeThreads / LANES;
+  __shared__ float4 s_acc[kMergeThreads];
+  __shared__ float2 s_ml[GROUPS];  // maximum and sum of each group
   pdl_wait();
   pdl_trigger();
-  const int b = blockIdx.x, h = blockIdx.y, rr = blockIdx.z, tid = threadIdx.x;
+  const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+  const int before = a.ws_pre[b], U = a.ws_pre[a.B];
   const SeqInfo sq = seq_info<ROWS>(a, b);
-  if (rr >= sq.n * a.G) return;
-  const int tok = rr / a.G, head = h * a.G + rr % a.G;
-  __nv_bfloat16* out = a.out + ((int64_t)(sq.q0 + tok) * a.Hq + head) * D + tid;
+  const int rows = sq.n * a.G;
+  const int grp = tid / LANES, lane = tid % LANES, d = lane * 4;
+  const int ways = rows < GROUPS ? GROUPS / max(rows, 1) : 1;  // groups that share a row
+  const int rr = ways > 1 ? grp / ways : blockIdx.z * GROUPS + grp, way = ways > 1 ? grp % ways : 0;
+  const bool on = rr < rows && (ways == 1 || blockIdx.z == 0);
+  if (ways > 1 && blockIdx.z > 0) return;
+  uint2* out = on ? reinterpret_cast<uint2*>(a.out + ((int64_t)(sq.q0 + rr / a.G) * a.Hq + h * a.G + rr % a.G) * D + d)
+                  : nullptr;
   if (sq.pages <= 0) {
-    *out = __float2bfloat16(0.f);
+    if (on) *out = make_uint2(0, 0);
     return;
   }
-  int64_t before = 0, all = 0;
-  for (int i = tid; i < a.B; i += D) {
-    const SeqInfo s = seq_info<ROWS>(a, i);
-    const int64_t n = (int64_t)a.Hkv * s.rb * s.pages;
-    all += n;
-    if (i < b) before += n;
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if ((tid & 31) == 0) {
-    s_sum[0][tid >> 5] = before;
-    s_sum[1][tid >> 5] = all;
-  }
-  __syncthreads();
-  before = all = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    before += s_sum[0][w];
-    all += s_sum[1][w];
-  }
-  const int64_t U = all, N = active_ctas(U, grid);
   const int rb = rr / ROWS, r = rr % ROWS;
-  const int64_t s0 = before + ((int64_t)h * sq.rb + rb) * sq.pages, s1 = s0 + sq.pages;
-  const int64_t i0 = ((s0 + 1) * N - 1) / U, i1 = (s1 * N - 1) / U;  // first and last CTA of the segment
-  if (i0 == i1) return;
-  auto part = [&](int64_t i) {
-    return a.ws + (i * 2 + (s0 < cta_begin(i, U, N) ? 0 : 1)) * ROWS * (D + 2);
-  };
-  float mx = -INFINITY;
-  for (int64_t i = i0 + (tid & 31); i <= i1; i += 32) mx = fmaxf(mx, part(i)[ROWS * D + r]);
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float sk2 = a.sinks != nullptr ? a.sinks[head] * kLog2e : -INFINITY;
-  const float top = fmaxf(mx, sk2);
-  float acc = 0.f, sum = sk2 == -INFINITY ? 0.f : ex2(sk2 - top);
-#pragma unroll 4
-  for (int64_t i = i0; i <= i1; ++i) {
-    const float* p = part(i);
-    const float mi = p[ROWS * D + r];
-    const float f = mi == -INFINITY ? 0.f : ex2(mi - top);
-    sum += f * p[ROWS * D + ROWS + r];
-    acc += f * p[r * D + tid];
+  const int s0 = before + (h * sq.rb + rb) * sq.pages, s1 = s0 + sq.pages;
+  const int chunk = warp_units(U, grid);
+  const int i0 = s0 / chunk, i1 = (s1 - 1) / chunk;  // first and last warp of the segment
+  const bool join = on && i0 != i1;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f, sink = 0.f, m_own = kNone;
+  if (join) {
+    // the first warp ends inside the segment, the others begin inside it
+    auto part = [&](int i) { return a.ws + ((int64_t)i * 2 + (i == i0 ? 1 : 0)) * ROWS * (D + 2); };
+    float top = a.sinks != nullptr ? a.sinks[h * a.G + rr % a.G] * kLog2e : kNone;
+    sink = a.sinks != nullptr ? 1.f : 0.f;  // the sink's weight, and the sums, relative to 2^top
+    constexpr int BATCH = 4;                // parts loaded at once: few rounds of latency
+    for (int i = i0 + way; i <= i1; i += BATCH * ways) {
+      float pm[BATCH], pl[BATCH];
+      float4 v[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const bool there = i + k * ways <= i1;
+        const float* p = part(there ? i + k * ways : i);
+        pm[k] = there ? p[ROWS * D + r] : kNone;
+        pl[k] = there ? p[ROWS * D + ROWS + r] : 0.f;
+        v[k] = *reinterpret_cast<const float4*>(p + r * D + d);
+      }
+      float mx = top;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) mx = fmaxf(mx, pm[k]);
+      const float f = ex2(top - mx);
+      sink *= f;
+      sum *= f;
+      acc.x *= f;
+      acc.y *= f;
+      acc.z *= f;
+      acc.w *= f;
+      top = mx;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const float w = i + k * ways <= i1 ? ex2(pm[k] - top) : 0.f;
+        sum += w * pl[k];
+        acc.x += w * v[k].x;
+        acc.y += w * v[k].y;
+        acc.z += w * v[k].z;
+        acc.w += w * v[k].w;
+      }
+    }
+    if (way == 0) sum += sink;
+    m_own = top;
   }
-  *out = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
+  if (ways > 1) {
+    s_acc[tid] = acc;
+    if (lane == 0) s_ml[grp] = make_float2(m_own, sum);
+    __syncthreads();
+    if (join && way == 0) {  // (rows * ways <= GROUPS: the groups of a row lie inside the arrays)
+      float top = m_own;
+      for (int w = 1; w < ways; ++w) top = fmaxf(top, s_ml[grp + w].x);
+      const float f0 = ex2(m_own - top);
+      sum *= f0;
+      acc.x *= f0;
+      acc.y *= f0;
+      acc.z *= f0;
+      acc.w *= f0;
+      for (int w = 1; w < ways; ++w) {
+        const float4 v = s_acc[tid + w * LANES];
+        const float2 ml = s_ml[grp + w];
+        const float f = ex2(ml.x - top);
+        sum += f * ml.y;
+        acc.x += f * v.x;
+        acc.y += f * v.y;
+        acc.z += f * v.z;
+        acc.w += f * v.w;
+      }
+    }
+  }
+  if (join && way == 0) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *out = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  }
 }
 
 }  // namespace kv8
@@ -836,10 +947,10 @@ namespace kv8 {
 static int tiles(int G, int max_q_len) { return std::min(4, (G * max_q_len + 7) / 8); }
 
 static int grid_ctas(int nt, int device, int B, int Hkv, int G, int max_q_len, int max_blocks) {
-  const int per_sm = nt == 1 ? 4 : (nt == 2 ? 3 : 2);
+  const int per_sm = 2;  // Cfg::CTAS
   const int64_t rb = ((int64_t)G * max_q_len + 8 * nt - 1) / (8 * nt);
   const int64_t units = (int64_t)B * Hkv * rb * max_blocks;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)per_sm * num_sms(device), (units + 3) / 4));
+  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)per_sm * num_sms(device), (units + 15) / 16));
 }
 
 template <int D, int NT>
@@ -852,20 +963,26 @@ static void run(const PagedInt8Args& a, int grid, cudaStream_t st) {
   auto k = attn_kernel<D, NT>;
   ensure_smem(k, smem);
   launch_pdl(k, dim3(grid), dim3(128), smem, st, tk, tv, a);
-  launch_pdl(merge_kernel<D, NT>, dim3(a.B, a.Hkv, a.G * a.max_q_len), dim3(D), 0, st, a, grid);
+  const int groups = kMergeThreads / (D / 4);
+  launch_pdl(merge_kernel<D, NT>, dim3(a.B, a.Hkv, (a.G * a.max_q_len + groups - 1) / groups), dim3(kMergeThreads), 0,
+             st, a, grid);
 }
 }  // namespace kv8
 
 int64_t paged_int8_ws_floats(int device, int B, int Hkv, int G, int D, int max_q_len, int max_blocks) {
   const int nt = kv8::tiles(G, max_q_len);
-  return (int64_t)kv8::grid_ctas(nt, device, B, Hkv, G, max_q_len, max_blocks) * 2 * 8 * nt * (D + 2);
+  return (int64_t)kv8::grid_ctas(nt, device, B, Hkv, G, max_q_len, max_blocks) * 4 * 2 * 8 * nt * (D + 2) + B + 1;
 }
 
-void paged_int8_launch(const PagedInt8Args& a, cudaStream_t st) {
+void paged_int8_launch(const PagedInt8Args& args, cudaStream_t st) {
   using namespace kv8;
+  PagedInt8Args a = args;
   if (a.B == 0 || a.T == 0 || a.max_q_len == 0) return;
   const int nt = tiles(a.G, a.max_q_len);
   const int grid = grid_ctas(nt, a.device, a.B, a.Hkv, a.G, a.max_q_len, a.max_blocks);
+  if ((int64_t)a.B * a.Hkv * (((int64_t)a.G * a.max_q_len + 8 * nt - 1) / (8 * nt)) * a.max_blocks > INT32_MAX / 2)
+    throw std::runtime_error("b200.paged_attention_int8: more pages in the batch than 2^30");
+  a.ws_pre = reinterpret_cast<int32_t*>(a.ws + (int64_t)grid * 4 * 2 * 8 * nt * (a.D + 2));
   if (a.D == 128) {
     if (nt == 1) run<128, 1>(a, grid, st);
     else if (nt == 2) run<128, 2>(a, grid, st);

@@ -378,7 +378,8 @@ struct PagedInt8Args {
   const int32_t* cu_q;      // [B + 1] query offsets, or null: one query per sequence
   __nv_bfloat16* out;       // [T, Hq, D]
   const float* sinks;       // [Hq] or null
-  float* ws;                // paged_int8_ws_floats() floats
+  float* ws;                // paged_int8_ws_floats() floats: two parts per warp, then ws_pre
+  int32_t* ws_pre = nullptr;  // [B + 1] (set by the launcher)
   int64_t num_blocks;
   int B, T, Hq, Hkv, G, D, max_blocks, max_q_len, window;
   float scale, softcap;
