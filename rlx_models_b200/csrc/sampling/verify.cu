@@ -11,9 +11,9 @@
 // Decisions are whole numbers, so what decides them is held in 64 bits: with
 // 1.5e5 tokens the borders of the running sum lie 1e-5 apart and closer, and sums
 // of 32-bit exponentials would move one draw in a thousand across a border.
-// exp_nonpos below costs about a dozen double-precision operations a logit, which
-// run under the loads of the logits (at 64 x 3.5 rows of 151936: 34 M logits,
-// 136 MB or 21 us of HBM, 23 us of double-precision arithmetic).
+// An exponential (Exp64) takes 8 double-precision operations, so 34 M logits (64
+// requests of 3.5 rows of 151936) are 15 us of the double-precision pipes under
+// the 21 us that their 136 MB take from HBM.
 //
 // Two launches. stats_kernel: one CTA per (row, 8192 logits) leaves the chunk's
 // maximum, sum of exponentials and argmax; rows are independent, so a single
@@ -21,6 +21,11 @@
 // sequence joins the chunks, accepts, and draws: every CTA sums its slice of w in
 // tiles of 512 tokens, the slice sums meet through distributed shared memory, and
 // the CTA whose slice holds the border walks its tiles.
+//
+// On a B200 a request with 4 drafts takes 18.5 us (the latency of the two launches
+// and a cluster's three meetings), 64 requests with up to 4 drafts 76 us: about 45
+// for the statistics, bound by instruction issue (29 a logit, 8 of them in 64 bits;
+// chunks of 4096 logits with more CTAs an SM are slower, 85 us in all).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -40,31 +45,68 @@ constexpr int kStatThreads = 256;
 constexpr int kPerThread = 32;
 constexpr int kChunk = kStatThreads * kPerThread;  // 8192
 constexpr int kCluster = 8;
-constexpr int kThreads = 256;
-constexpr int kTile = 512;  // tokens per warp step: 16 per lane
+constexpr int kLaneTile = 16;
+constexpr int kTile = 32 * kLaneTile;  // tokens per warp step
+constexpr int kRows = 32;              // rows whose statistics a CTA keeps
+constexpr float kMaxTemperature = 1e30f;
 
-// 2^(j / 64), filled once per CTA.
+constexpr int kTable = 512;
+
+// 2^(j / 512) by the Taylor series of e^(j ln 2 / 512), at compile time.
+struct Exp2Table {
+  double v[kTable];
+  constexpr Exp2Table() : v{} {
+    for (int j = 0; j < kTable; ++j) {
+      const double x = j * (0.693147180559945309417 / kTable);
+      double sum = 1.0;
+      for (int k = 24; k > 0; --k) sum = 1.0 + sum * x / k;
+      v[j] = sum;
+    }
+  }
+};
+__device__ constexpr Exp2Table kExp2Table{};
+
 __device__ __forceinline__ void fill_table(double* tab) {
-  for (int j = threadIdx.x; j < 64; j += blockDim.x) tab[j] = exp2((double)j * (1.0 / 64.0));
+  for (int j = threadIdx.x; j < kTable; j += blockDim.x) tab[j] = kExp2Table.v[j];
 }
 
-// e^x for x <= 0 given y = x * 64 / ln 2: y = 64 n + j + r with |r| <= 1/2, so
-// e^x = 2^n 2^(j / 64) e^z, z = r ln 2 / 64, |z| < 0.00542: Taylor to z^5 leaves
-// z^6 / 720 < 4e-17. Results below the normal range are 0.
-__device__ __forceinline__ double exp_nonpos(double y, const double* tab) {
-  const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are rint(y)
-  if (!(y > -64.0 * 1000.0)) return 0.0;
-  const double k = y + magic;
-  const int i = __double2loint(k);
-  const double z = (y - (k - magic)) * (0.693147180559945309417 / 64.0);
-  double e = fma(z, 1.0 / 120.0, 1.0 / 24.0);
-  e = fma(e, z, 1.0 / 6.0);
-  e = fma(e, z, 0.5);
-  e = fma(e, z, 1.0);
-  e = fma(e, z, 1.0);
-  const double r = tab[i & 63] * e;
-  return __hiloint2double(__double2hiint(r) + ((i >> 6) << 20), __double2loint(r));
-}
+// e^((x - max) / T) for x <= max in 64 bits: y = (x - max) 512 / (T ln 2) = 512 n + j + r with |r| <= 1/2, so the value
+// is 2^n 2^(j / 512) e^z, z = r ln 2 / 512, |z| < 0.00068; Taylor to z^3 leaves z^4 / 24 < 9e-15 of it. Terms below
+// e^-700 are 0 (`keep`), and so are those of -inf and NaN.
+struct Exp64 {
+  double f, c;  // y = f x + c
+  float max, cut;
+  const double* tab;
+  __device__ __forceinline__ Exp64(float mx, float T, const double* table)
+      : f(kTable * 1.44269504088896340736 / (double)T), c(-f * (double)mx), max(mx), cut(-700.f * T), tab(table) {}
+  __device__ __forceinline__ bool keep(float x) const { return x - max > cut; }
+  // scale * e^z without the range check
+  __device__ __forceinline__ void parts(float x, double& scale, double& e) const {
+    constexpr double ln = 0.693147180559945309417 / kTable, magic = 6755399441055744.0;  // 1.5 * 2^52
+    const double y = fma((double)x, f, c);
+    const double k = y + magic;  // the sum's low bits are rint(y)
+    const int i = __double2loint(k);
+    const double r = y - (k - magic);
+    e = fma(r, ln * ln * ln / 6.0, ln * ln / 2.0);
+    e = fma(e, r, ln);
+    e = fma(e, r, 1.0);
+    const double t = tab[i & (kTable - 1)];
+    scale = __hiloint2double(__double2hiint(t) + ((i >> 9) << 20), __double2loint(t));
+  }
+  __device__ __forceinline__ void add(float x, double& sum) const {  // of a term that is kept
+    double scale, e;
+    parts(x, scale, e);
+    sum = fma(scale, e, sum);
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    double scale, e;
+    parts(x, scale, e);
+    return keep(x) ? scale * e : 0.0;
+  }
+};
+
+__device__ __forceinline__ bool sampled(float T) { return T > 0.f; }
+__device__ __forceinline__ float bounded(float T) { return T > kMaxTemperature ? kMaxTemperature : T; }  // (keeps NaN)
 
 // NaN logits are never chosen, +inf counts as the largest finite number.
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
@@ -74,29 +116,20 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// last b with cu_rows[b] <= row
-__device__ __forceinline__ int seq_of(const int32_t* cu, int B, int row) {
-  int lo = 0, hi = B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-__global__ void __launch_bounds__(kStatThreads) stats_kernel(VerifyArgs a) {
-  __shared__ double tab[64];
+__global__ void __launch_bounds__(kStatThreads, 4) stats_kernel(VerifyArgs a) {
+  __shared__ double tab[kTable];
   __shared__ float s_max[kStatThreads / 32];
   __shared__ int s_arg[kStatThreads / 32];
   __shared__ double s_sum[kStatThreads / 32];
+  __shared__ float s_t;
   fill_table(tab);
   pdl_wait();
   pdl_trigger();
   const int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x;
-  const float T = a.temperature[seq_of(a.cu_rows, a.B, row)];
   const float* x = a.logits + (int64_t)row * a.ld;
   const int lo = chunk * kChunk, hi = min(lo + kChunk, a.V);
+  if (tid == 0) s_t = 0.f;  // (a row of no sequence)
+  __syncthreads();
   float v[kPerThread];
   if ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && hi - lo == kChunk) {
 #pragma unroll
@@ -114,15 +147,23 @@ __global__ void __launch_bounds__(kStatThreads) stats_kernel(VerifyArgs a) {
       v[i] = at < hi ? x[at] : -INFINITY;
     }
   }
+  for (int b = tid; b < a.B; b += kStatThreads)  // the row's sequence: one round of loads, beside those of the logits
+    if (a.cu_rows[b] <= row && row < a.cu_rows[b + 1]) s_t = a.temperature[b];
   float best = -INFINITY;
-  int arg = 0x7fffffff;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    v[i] = clean(v[i]);
-    if (v[i] > best) {
-      best = v[i];
-      arg = lo + ((i >> 2) * kStatThreads + tid) * 4 + (i & 3);
-    }
+  for (int i = 0; i < kPerThread; ++i) best = fmaxf(best, v[i]);  // (NaN loses)
+  if (best == INFINITY) {  // +inf counts as the largest finite number
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) v[i] = clean(v[i]);
+    best = FLT_MAX;
+  }
+  __syncthreads();
+  const float T = bounded(s_t);
+  int arg = 0x7fffffff;
+  if (!sampled(T)) {
+#pragma unroll
+    for (int i = kPerThread - 1; i >= 0; --i)
+      if (v[i] == best && best != -INFINITY) arg = lo + ((i >> 2) * kStatThreads + tid) * 4 + (i & 3);
   }
   for (int o = 16; o > 0; o >>= 1) {
     const float ob = __shfl_xor_sync(0xffffffffu, best, o);
@@ -147,10 +188,18 @@ __global__ void __launch_bounds__(kStatThreads) stats_kernel(VerifyArgs a) {
     }
   }
   double sum = 0.0;
-  if (T > 0.f && best != -INFINITY) {
-    const double f = 64.0 * 1.44269504088896340736 / (double)T;
+  if (sampled(T) && best != -INFINITY) {
+    const Exp64 ex(best, T, tab);
+    double part[2] = {0.0, 0.0};
+    const float low = best + ex.cut;
+    if (low < best) {  // terms below the cut enter as e^-700, which no sum of 1 and more sees (NaN loses)
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) sum += exp_nonpos(((double)v[i] - (double)best) * f, tab);
+      for (int i = 0; i < kPerThread; ++i) ex.add(fmaxf(v[i], low), part[i & 1]);
+    } else {  // so cold that only the maximum counts
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i) part[0] += v[i] == best ? 1.0 : 0.0;
+    }
+    sum = part[0] + part[1];
   }
   sum = warp_sum(sum);
   if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
@@ -172,15 +221,17 @@ struct RowStat {
 };
 
 // One warp: the chunks of a row joined (every lane gets the result).
-__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, int64_t row, double f, const double* tab) {
+__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, int64_t row, float T, const double* tab) {
   const int lane = threadIdx.x & 31;
+  const float* pm = a.part_max + row * a.chunks;
   float best = -INFINITY;
   int arg = 0x7fffffff;
   for (int c = lane; c < a.chunks; c += 32) {
-    const float m = a.part_max[row * a.chunks + c];
+    const float m = pm[c];
+    const int i = a.part_arg[row * a.chunks + c];
     if (m > best) {
       best = m;
-      arg = a.part_arg[row * a.chunks + c];
+      arg = i;
     }
   }
   for (int o = 16; o > 0; o >>= 1) {
@@ -192,21 +243,24 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, int64_t row, do
     }
   }
   double sum = 0.0;
-  if (best != -INFINITY)
-    for (int c = lane; c < a.chunks; c += 32)
-      sum += a.part_sum[row * a.chunks + c] *
-             exp_nonpos(((double)a.part_max[row * a.chunks + c] - (double)best) * f, tab);
+  if (sampled(T) && best != -INFINITY) {
+    const Exp64 ex(best, T, tab);
+    for (int c = lane; c < a.chunks; c += 32) sum += a.part_sum[row * a.chunks + c] * ex(pm[c]);
+  }
   return {best, warp_sum(sum), arg};
 }
 
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) decide_kernel(VerifyArgs a) {
+template <int kThreads, int kBlocks>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, kBlocks) decide_kernel(VerifyArgs a) {
+  constexpr int kWarps = kThreads / 32;
   extern __shared__ double tiles[];  // sums of this CTA's tiles
-  __shared__ double tab[64];
+  __shared__ double tab[kTable];
   __shared__ double s_slice;         // sum of w over this CTA's slice
-  __shared__ RowStat s_row;
-  __shared__ double s_p;
-  __shared__ int s_count, s_tok, s_last;
+  __shared__ RowStat s_row[kRows];
+  __shared__ double s_before;
+  __shared__ int s_count, s_tile, s_end;
   cg::cluster_group cluster = cg::this_cluster();
+  if (threadIdx.x == 0) s_count = 0x7fffffff;
   fill_table(tab);
   pdl_wait();
   pdl_trigger();
@@ -216,39 +270,40 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) dec
   const int64_t r1 = min(max((int64_t)a.cu_rows[b + 1], r0), a.R);
   const int n = (int)min(r1 - r0 - 1, (int64_t)a.max_drafts);  // drafts; < 0: the sequence has no rows
   int32_t* out = a.tokens + (int64_t)b * (a.max_drafts + 1);
-  const float T = a.temperature[b];
-  const double f = T > 0.f ? 64.0 * 1.44269504088896340736 / (double)T : 0.0;
+  const float T = bounded(a.temperature[b]);
   const int64_t d0 = r0 - b;
   __syncthreads();
 
-  // acceptance: one warp per drafted row, then the first refusal counts
-  if (tid == 0) s_count = max(n, 0);
-  __syncthreads();
-  for (int i = warp; i < n; i += kThreads / 32) {
+  // acceptance: one warp per row; the first refusal counts
+  for (int i = warp; i <= n; i += kWarps) {
     const int64_t di = d0 + i;
-    const int tok = di >= 0 && di < a.ND ? a.drafts[di] : -1;
-    const RowStat st = row_stat(a, r0 + i, f, tab);
+    const int tok = i < n && di >= 0 && di < a.ND ? a.drafts[di] : -1;
+    const bool token = tok >= 0 && tok < a.V;
+    const float x = token ? clean(a.logits[(r0 + i) * a.ld + tok]) : 0.f;
+    const float q = token && a.probs != nullptr ? a.probs[di * a.ldp + tok] : 1.f;
+    const RowStat st = row_stat(a, r0 + i, T, tab);
+    if (lane == 0 && i < kRows) s_row[i] = st;
     bool ok = false;
-    if (tok >= 0 && tok < a.V) {
-      if (!(T > 0.f)) {
+    if (token) {
+      if (!sampled(T)) {
         ok = tok == st.arg;
       } else if (st.max != -INFINITY) {
-        const float x = clean(a.logits[(r0 + i) * a.ld + tok]);
-        const double p = exp_nonpos(((double)x - (double)st.max) * f, tab) / st.sum;
-        const float q = a.probs != nullptr ? a.probs[di * a.ldp + tok] : 1.f;
+        const double p = Exp64(st.max, T, tab)(x) / st.sum;
         ok = (double)a.uniforms[r0 + i] * (double)(q > 0.f ? q : 0.f) < p;
       }
     }
-    if (lane == 0 && !ok) atomicMin(&s_count, i);
+    if (lane == 0 && i < n && !ok) atomicMin(&s_count, i);
   }
   __syncthreads();
-  const int count = s_count;
+  const int count = min(s_count, max(n, 0));
   const int64_t row = r0 + count;
-  if (warp == 0 && n >= 0) {
-    const RowStat st = row_stat(a, row, f, tab);
-    if (lane == 0) s_row = st;
+  if (n >= 0 && count >= kRows) {
+    if (warp == 0) {
+      const RowStat st = row_stat(a, row, T, tab);
+      if (lane == 0) s_row[0] = st;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (rank == 0) {
     if (tid == 0) a.accepted[b] = count;
     for (int i = tid; i <= a.max_drafts; i += kThreads) {
@@ -257,51 +312,61 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) dec
     }
   }
   if (n < 0) return;  // the whole cluster alike
-  const RowStat st = s_row;
-  if (!(T > 0.f) || st.max == -INFINITY) {  // argmax (0 for a row without a finite logit, as ops.argmax)
+  const RowStat st = s_row[count < kRows ? count : 0];
+  if (!sampled(T) || st.max == -INFINITY) {  // argmax (0 for a row without a finite logit, as ops.argmax)
     if (rank == 0 && tid == 0) out[count] = st.max == -INFINITY ? 0 : st.arg;
     return;
   }
 
-  // w over this CTA's slice, tile by tile
+  // w over this CTA's slice, tile by tile; the loads of a tile are on their way together
   const float* x = a.logits + row * a.ld;
   const int64_t di = d0 + count;
   const bool rejected = count < n && di >= 0 && di < a.ND;  // (a draft outside its list: drawn from p)
   const float* q = rejected && a.probs != nullptr ? a.probs + di * a.ldp : nullptr;
   const int gone = rejected && a.probs == nullptr ? a.drafts[di] : -1;  // a certain draft: q = 1 there
-  const double inv = 1.0 / st.sum, mx = (double)st.max;
-  auto weight = [&](int i, bool plain) -> double {
-    double w = exp_nonpos(((double)clean(x[i]) - mx) * f, tab) * inv;
-    if (!plain) {
-      if (q != nullptr) {
-        const float qi = q[i];
-        w = fmax(w - (double)(qi > 0.f ? qi : 0.f), 0.0);
-      }
-      if (i == gone) w = 0.0;
+  const double inv = 1.0 / st.sum;
+  const Exp64 ex(st.max, T, tab);
+  bool plain = !rejected;
+  auto tile_weights = [&](int t, auto&& use) {  // use(i, w) of tokens t * kTile + i * 32 + lane
+    float xv[kLaneTile], qv[kLaneTile];
+#pragma unroll
+    for (int i = 0; i < kLaneTile; ++i) {
+      const int at = t * kTile + i * 32 + lane;
+      xv[i] = at < a.V ? x[at] : -INFINITY;
     }
-    return w;
+#pragma unroll
+    for (int i = 0; i < kLaneTile; ++i) {
+      const int at = t * kTile + i * 32 + lane;
+      qv[i] = !plain && q != nullptr && at < a.V ? q[at] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kLaneTile; ++i) {
+      const float xi = clean(xv[i]);
+      double scale, e;
+      ex.parts(xi, scale, e);
+      const double v = fma(scale * e, inv, -(double)(qv[i] > 0.f ? qv[i] : 0.f));
+      const bool on = ex.keep(xi) && (plain || t * kTile + i * 32 + lane != gone);
+      use(i, on && v > 0.0 ? v : 0.0);
+    }
   };
   const int all_tiles = (a.V + kTile - 1) / kTile;
   const int per = (all_tiles + kCluster - 1) / kCluster;
-  const int tile0 = min(rank * per, all_tiles), tile1 = min(tile0 + per, all_tiles);
-  bool plain = !rejected;
+  const int tile0 = min(rank * per, all_tiles), mine = min(tile0 + per, all_tiles) - tile0;
+  const int seg = (mine + 31) / 32;  // tiles per lane, in order, where one warp adds them up
   double total = 0.0;
   for (int pass = 0; pass < 2; ++pass) {
-    for (int t = tile0 + warp; t < tile1; t += kThreads / 32) {
-      double sum = 0.0;
-#pragma unroll 4
-      for (int i = 0; i < kTile / 32; ++i) {
-        const int at = t * kTile + i * 32 + lane;
-        if (at < a.V) sum += weight(at, plain);
-      }
-      sum = warp_sum(sum);
-      if (lane == 0) tiles[t - tile0] = sum;
+    for (int t = warp; t < mine; t += kWarps) {
+      double part[2] = {0.0, 0.0};
+      tile_weights(tile0 + t, [&](int i, double w) { part[i & 1] += w; });
+      const double sum = warp_sum(part[0] + part[1]);
+      if (lane == 0) tiles[t] = sum;
     }
     __syncthreads();
-    if (tid == 0) {
+    if (warp == 0) {
       double s = 0.0;
-      for (int t = 0; t < tile1 - tile0; ++t) s += tiles[t];
-      s_slice = s;
+      for (int t = lane * seg; t < min(lane * seg + seg, mine); ++t) s += tiles[t];
+      s = warp_sum(s);
+      if (lane == 0) s_slice = s;
     }
     cluster.sync();
     total = 0.0;
@@ -312,9 +377,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) dec
   }
   const double target = (double)a.uniforms[r1 - 1] * total;
   // the slice that the border lies in; behind every border (rounding): the last slice with weight
-  double before = 0.0;
+  double before = 0.0, owner_before = 0.0;
   int owner = -1, fallback = 0;
-  double owner_before = 0.0;
   for (int c = 0; c < kCluster; ++c) {
     const double s = *cluster.map_shared_rank(&s_slice, c);
     if (s > 0.0) fallback = c;
@@ -325,47 +389,55 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) dec
     before += s;
   }
   const bool end = owner < 0;  // take the last token with weight of the fallback slice
-  if (end) owner = fallback;
-  if (rank == owner) {
-    if (tid == 0) {
-      double s = owner_before;
-      int pick = -1, last = 0;
-      for (int t = 0; t < tile1 - tile0; ++t) {
-        if (tiles[t] > 0.0) last = t;
-        if (!end && s + tiles[t] > target) {
-          pick = t;
-          break;
-        }
-        s += tiles[t];
-      }
-      s_tok = pick >= 0 ? pick : last;
-      s_p = s;
-      s_last = pick < 0 ? 1 : 0;
+  if (rank == (end ? fallback : owner) && warp == 0) {
+    // the tile: a running sum over the lanes' tiles, then over the tiles of the lane that holds the border
+    double s = 0.0;
+    int last = -1;
+    for (int t = lane * seg; t < min(lane * seg + seg, mine); ++t) {
+      s += tiles[t];
+      if (tiles[t] > 0.0) last = t;
     }
-    __syncthreads();
-    if (warp == 0) {
-      const int t = tile0 + s_tok;
-      double s = s_p;
-      int chosen = -1, last = 0;
-      for (int i = 0; i < kTile / 32; ++i) {
-        const int at = t * kTile + i * 32 + lane;
-        const double w = at < a.V ? weight(at, plain) : 0.0;
-        double inc = w;
-        for (int o = 1; o < 32; o <<= 1) {
-          const double v = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += v;
-        }
-        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-        if (some != 0) last = t * kTile + i * 32 + 31 - __clz(some);
-        const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && s + inc > target);
-        if (hit != 0 && s_last == 0) {
-          chosen = t * kTile + i * 32 + __ffs(hit) - 1;
-          break;
-        }
-        s += __shfl_sync(0xffffffffu, inc, 31);
-      }
-      if (lane == 0) out[count] = chosen >= 0 ? chosen : last;
+    double inc = s;
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
     }
+    const unsigned hit = end ? 0u : __ballot_sync(0xffffffffu, last >= 0 && owner_before + inc > target);
+    for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+    if (lane == (hit != 0 ? __ffs(hit) - 1 : 0)) {
+      s_tile = last;
+      s_end = 1;
+      s_before = 0.0;
+      if (hit != 0) {
+        double run = owner_before + inc - s;
+        int pick = -1;
+        for (int t = lane * seg; t < min(lane * seg + seg, mine); ++t) {
+          if (tiles[t] > 0.0) pick = t;  // (rounding: the last one with weight holds it)
+          if (run + tiles[t] > target) break;
+          if (t + 1 < min(lane * seg + seg, mine)) run += tiles[t];
+        }
+        s_tile = pick;
+        s_end = 0;
+        s_before = run;
+      }
+    }
+    __syncwarp();
+    const int t = tile0 + s_tile;
+    double sum = s_before;
+    int chosen = -1, tail = 0;
+    tile_weights(t, [&](int i, double w) {
+      double run = w;
+      for (int o = 1; o < 32; o <<= 1) {
+        const double v = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += v;
+      }
+      const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
+      if (some != 0) tail = t * kTile + i * 32 + 31 - __clz(some);
+      const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && sum + run > target);
+      if (over != 0 && s_end == 0 && chosen < 0) chosen = t * kTile + i * 32 + __ffs(over) - 1;
+      sum += __shfl_sync(0xffffffffu, run, 31);
+    });
+    if (lane == 0) out[count] = chosen >= 0 ? chosen : tail;
   }
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }
@@ -380,7 +452,11 @@ void verify_drafts_launch(const VerifyArgs& a, cudaStream_t st) {
   if (a.R > 0) launch_pdl(stats_kernel, dim3((unsigned)a.chunks, (unsigned)a.R), dim3(kStatThreads), 0, st, a);
   const int all_tiles = (a.V + kTile - 1) / kTile;
   const size_t smem = (size_t)((all_tiles + kCluster - 1) / kCluster) * sizeof(double);
-  launch_pdl(decide_kernel, dim3((unsigned)a.B * kCluster), dim3(kThreads), smem, st, a);
+  // few sequences: more warps on each, the time is the latency of a cluster; many: 4 CTAs an SM hide it from one another
+  if (a.B <= 16)
+    launch_pdl(decide_kernel<512, 2>, dim3((unsigned)a.B * kCluster), dim3(512), smem, st, a);
+  else
+    launch_pdl(decide_kernel<256, 4>, dim3((unsigned)a.B * kCluster), dim3(256), smem, st, a);
 }
 
 }  // namespace b200
