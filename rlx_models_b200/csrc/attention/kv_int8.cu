@@ -65,68 +65,83 @@ __global__ void __launch_bounds__(kStoreWarps * 32) store_kernel(KvInt8StoreArgs
   int8_t* codes = is_v ? a.v_cache : a.k_cache;
   float* scales = is_v ? a.v_scale : a.k_scale;
 
-  for (int64_t t = t0; t < t1; ++t) {
-    const int64_t slot = a.slots[t];
-    if (slot < 0) continue;
-    const int64_t blk = slot >> 4;
-    if (t > 0) {  // only the first token of a run of one block works
-      const int64_t prev = a.slots[t - 1];
-      if (prev >= 0 && (prev >> 4) == blk) continue;
-    }
+  // slots of the group and behind it (lane i: token t0 + i), and the first tokens of the runs in the group
+  const int64_t near = t0 + lane < a.T ? a.slots[t0 + lane] : -1;
+  int64_t ahead = __shfl_up_sync(0xffffffffu, near, 1);
+  if (lane == 0) ahead = t0 > 0 ? a.slots[t0 - 1] : -1;
+  unsigned firsts =
+      __ballot_sync(0xffffffffu, t0 + lane < t1 && near >= 0 && (ahead < 0 || (ahead >> 4) != (near >> 4)));
+  while (firsts != 0) {
+    const int at = __ffs(firsts) - 1;
+    firsts &= firsts - 1;
+    const int64_t blk = __shfl_sync(0xffffffffu, near, at) >> 4;
     if (blk >= a.num_blocks) {
       if (lane == 0) report_error(a.status, kErrBounds, (int)min(blk, (int64_t)0x7fffffff));
       continue;
     }
+    const int64_t page = blk * a.Hkv + h;
+    const float old = scales[page];  // (asked for early; used when the block is not new)
     // lane o < 16: newest token of the run written at offset o (-1: none)
     int64_t src = -1;
-    for (int64_t base = t;; base += 32) {
-      const int64_t tt = base + lane;
-      const int64_t s = tt < a.T ? a.slots[tt] : -1;
-      const bool same = s >= 0 && (s >> 4) == blk;
-      const unsigned in = __ballot_sync(0xffffffffu, same);
-      const int len = in == 0xffffffffu ? 32 : __ffs(~in) - 1;  // tokens of the run in this chunk
-      const int off = (int)(s & 15);
-#pragma unroll
-      for (int o = 0; o < 16; ++o) {
-        const unsigned m = __ballot_sync(0xffffffffu, lane < len && off == o);
-        if (lane == o && m != 0) src = base + (31 - __clz(m));
+    int64_t slot = __shfl_down_sync(0xffffffffu, near, at);
+    int span = 32 - at;  // lanes with a slot of this piece of the run
+    for (int64_t base = t0 + at;;) {
+      const unsigned in = __ballot_sync(0xffffffffu, lane < span && slot >= 0 && (slot >> 4) == blk);
+      const int len = in == 0xffffffffu ? 32 : __ffs(~in) - 1;  // tokens of the run in this piece
+      const int off = lane < len ? (int)(slot & 15) : 16 + lane;
+      const unsigned same = __match_any_sync(0xffffffffu, off);  // tokens of one offset: the last one counts
+      for (unsigned todo = __ballot_sync(0xffffffffu, off < 16 && (same >> lane) == 1u); todo != 0; todo &= todo - 1) {
+        const int from = __ffs(todo) - 1;
+        if (lane == __shfl_sync(0xffffffffu, off, from)) src = base + from;
       }
-      if (len < 32) break;
+      if (len < span) break;
+      base += span;
+      span = 32;
+      slot = base + lane < a.T ? a.slots[base + lane] : -1;
     }
     const bool fresh = __shfl_sync(0xffffffffu, src, 0) >= 0;
-    const int64_t page = (blk * a.Hkv + h);
     const int c = (lane % CPR) * 16;
     uint4 lo[NI], hi[NI];
     bool given[NI];
-    uint32_t amax = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = lane / CPR + i * RPW;
       const int64_t st = __shfl_sync(0xffffffffu, src, r);
       given[i] = st >= 0;
+      lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
       if (given[i]) {
         const uint4* p = reinterpret_cast<const uint4*>(x + st * xt + h * xh + c);
         lo[i] = p[0];
         hi[i] = p[1];
       }
     }
+    // magnitudes of bf16 order like their bits
+    uint32_t amax2 = 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      if (given[i]) {
+      const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax2 = __vmaxu2(amax2, w[j] & 0x7fff7fffu);
+    }
+    uint32_t amax = __reduce_max_sync(0xffffffffu, max(amax2 & 0xffffu, amax2 >> 16));
+    const bool finite = amax < 0x7f80u;
+    if (!finite) {  // infinities and NaN do not count
+      amax = 0;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
         const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {  // magnitudes of bf16 order like their bits; infinities and NaN do not count
+        for (int j = 0; j < 8; ++j) {
           const uint32_t u = w[j] & 0x7fffu, v = (w[j] >> 16) & 0x7fffu;
           amax = max(amax, max(u < 0x7f80u ? u : 0u, v < 0x7f80u ? v : 0u));
         }
       }
+      amax = __reduce_max_sync(0xffffffffu, amax);
     }
-    amax = __reduce_max_sync(0xffffffffu, amax);
     // amax = (1 + m / 128) 2^E <= 127 * 2^e = (1 + 126 / 128) 2^(e + 6)
     const int e = max((int)(amax >> 7) - 127 - 6 + ((amax & 127u) == 127u ? 1 : 0), kMinExp);
     float s = __int_as_float((e + 127) << 23), ratio = 0.f;
     if (!fresh) {
-      const float old = scales[page];
       s = fmaxf(s, old);
       ratio = old / s;
     }
@@ -141,12 +156,16 @@ __global__ void __launch_bounds__(kStoreWarps * 32) store_kernel(KvInt8StoreArgs
         const uint32_t w[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          // __float2int_rn: ties to even, NaN -> 0, infinities saturate (then clamp)
-          const int q0 = max(-127, min(127, __float2int_rn(bf16_lo(w[2 * j]) * inv)));
-          const int q1 = max(-127, min(127, __float2int_rn(bf16_hi(w[2 * j]) * inv)));
-          const int q2 = max(-127, min(127, __float2int_rn(bf16_lo(w[2 * j + 1]) * inv)));
-          const int q3 = max(-127, min(127, __float2int_rn(bf16_hi(w[2 * j + 1]) * inv)));
-          o[j] = __byte_perm(__byte_perm(q0, q1, 0x0040), __byte_perm(q2, q3, 0x0040), 0x5410);
+          float f[4] = {bf16_lo(w[2 * j]), bf16_hi(w[2 * j]), bf16_lo(w[2 * j + 1]), bf16_hi(w[2 * j + 1])};
+          if (!finite) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = f[k] != f[k] ? 0.f : fminf(fmaxf(f[k], -127.f * s), 127.f * s);
+          }
+          // x / s is exact, so that adding 1.5 * 2^23 rounds it once, ties to even: the code is the low byte
+          uint32_t q[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) q[k] = __float_as_uint(fmaf(f[k], inv, 12582912.f));
+          o[j] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
         }
       } else if (fresh) {
         o[0] = o[1] = o[2] = o[3] = 0;
@@ -186,36 +205,48 @@ __device__ __forceinline__ uint2 widen_bf16(uint32_t w, float s) {
   return make_uint2(pack_bf16x2(f0, f1), pack_bf16x2(f2, f3));
 }
 
-// One CTA per (sequence, page): every KV head, K and V. 1 byte read and 2
-// written per element: bound by HBM.
-__global__ void __launch_bounds__(256) dequant_kernel(KvInt8DequantArgs a) {
+// One CTA per (sequence, page, quarter of its heads' codes): 16 codes a thread
+// and step, up to four steps' loads in flight. 1 byte read and 2 written per
+// element: bound by HBM.
+constexpr int kDequantThreads = 128, kDequantSteps = 4;
+
+__global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantArgs a) {
   pdl_wait();
   pdl_trigger();
   const int b = blockIdx.x / a.max_blocks, p = blockIdx.x % a.max_blocks;
-  const int ctx = a.ctx_lens[b];
+  const int id = a.tables[blockIdx.x], ctx = a.ctx_lens[b];
+  if (a.table_out != nullptr && blockIdx.y == 0 && threadIdx.x == 0) a.table_out[blockIdx.x] = blockIdx.x;
   if (p * 16 >= ctx && p > 0) return;
-  const int64_t id = a.tables[(int64_t)b * a.max_blocks + p];
   const bool known = id >= 0 && id < a.num_blocks && ctx > 0;
-  if (!known && ctx > 0 && threadIdx.x == 0) report_error(a.status, kErrBounds, (int)id);
+  if (!known && ctx > 0 && threadIdx.x == 0) report_error(a.status, kErrBounds, id);
   const int head = 16 * a.D, n = a.Hkv * head;
-  const int64_t dst = (int64_t)blockIdx.x * n;
-  if (!known) {  // the first page of an empty sequence, which attention may still load, and pages that do not exist
-    for (int i = threadIdx.x * 8; i < n; i += 256 * 8) {
-      *reinterpret_cast<uint4*>(a.k_out + dst + i) = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(a.v_out + dst + i) = make_uint4(0, 0, 0, 0);
+  const int64_t src = (int64_t)id * n, dst = (int64_t)blockIdx.x * n;
+  const int j0 = (blockIdx.y * kDequantSteps * kDequantThreads + threadIdx.x) * 16;
+  uint4 w[kDequantSteps];
+  float s[kDequantSteps];
+#pragma unroll
+  for (int k = 0; k < kDequantSteps; ++k) {  // K codes, then V codes
+    const int j = j0 + k * kDequantThreads * 16;
+    w[k] = make_uint4(0, 0, 0, 0);
+    s[k] = 0.f;  // the first page of an empty sequence, which attention may still load, and unknown pages hold zeros
+    if (known && j < 2 * n) {
+      const bool is_v = j >= n;
+      const int c = is_v ? j - n : j;
+      w[k] = __ldcs(reinterpret_cast<const uint4*>((is_v ? a.v_cache : a.k_cache) + src + c));
+      s[k] = (is_v ? a.v_scale : a.k_scale)[(int64_t)id * a.Hkv + c / head];
     }
-    return;
   }
-  for (int i = threadIdx.x * 16; i < 2 * n; i += 256 * 16) {
-    const bool is_v = i >= n;
-    const int j = is_v ? i - n : i;
-    const int8_t* codes = is_v ? a.v_cache : a.k_cache;
-    const float s = (is_v ? a.v_scale : a.k_scale)[id * a.Hkv + j / head];
-    const uint4 w = *reinterpret_cast<const uint4*>(codes + id * n + j);
-    __nv_bfloat16* out = (is_v ? a.v_out : a.k_out) + dst + j;
-    const uint2 x = widen_bf16(w.x, s), y = widen_bf16(w.y, s), z = widen_bf16(w.z, s), u = widen_bf16(w.w, s);
-    reinterpret_cast<uint4*>(out)[0] = make_uint4(x.x, x.y, y.x, y.y);
-    reinterpret_cast<uint4*>(out)[1] = make_uint4(z.x, z.y, u.x, u.y);
+#pragma unroll
+  for (int k = 0; k < kDequantSteps; ++k) {
+    const int j = j0 + k * kDequantThreads * 16;
+    if (j < 2 * n) {
+      const bool is_v = j >= n;
+      __nv_bfloat16* out = (is_v ? a.v_out : a.k_out) + dst + (is_v ? j - n : j);
+      const uint2 x = widen_bf16(w[k].x, s[k]), y = widen_bf16(w[k].y, s[k]);
+      const uint2 z = widen_bf16(w[k].z, s[k]), u = widen_bf16(w[k].w, s[k]);
+      reinterpret_cast<uint4*>(out)[0] = make_uint4(x.x, x.y, y.x, y.y);
+      reinterpret_cast<uint4*>(out)[1] = make_uint4(z.x, z.y, u.x, u.y);
+    }
   }
 }
 
@@ -939,7 +970,10 @@ void kv_int8_store_launch(const KvInt8StoreArgs& args, int D, cudaStream_t st) {
 
 void kv_int8_dequant_launch(const KvInt8DequantArgs& a, cudaStream_t st) {
   if (a.B == 0 || a.max_blocks == 0) return;
-  launch_pdl(kv8::dequant_kernel, dim3((unsigned)(a.B * a.max_blocks)), dim3(256), 0, st, a);
+  const int per_cta = kv8::kDequantThreads * kv8::kDequantSteps * 16;
+  const int parts = (2 * a.Hkv * 16 * a.D + per_cta - 1) / per_cta;
+  launch_pdl(kv8::dequant_kernel, dim3((unsigned)(a.B * a.max_blocks), (unsigned)parts), dim3(kv8::kDequantThreads), 0,
+             st, a);
 }
 
 namespace kv8 {

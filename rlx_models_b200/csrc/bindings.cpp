@@ -674,19 +674,18 @@ static void check_int8_tables(const char* op, const Tensor& k_cache, const Tenso
   TORCH_CHECK(tables.size(1) < (1 << 27), "b200.", op, ": block_tables too wide");
 }
 
-void kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
-                           const Tensor& block_tables, const Tensor& ctx_lens, Tensor& k_out, Tensor& v_out,
-                           Tensor& status) {
+std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
+                                          const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
+                                          Tensor& status) {
   check_int8_cache("kv_dequant_pages_int8", k_cache, v_cache, k_scale, v_scale);
   check_int8_tables("kv_dequant_pages_int8", k_cache, block_tables, ctx_lens);
   const int64_t B = block_tables.size(0), mb = block_tables.size(1);
   TORCH_CHECK(B * mb <= INT32_MAX, "b200.kv_dequant_pages_int8: block_tables too large");
-  for (const Tensor* t : {&k_out, &v_out})
-    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->is_contiguous() && t->dim() == 4 && t->size(0) >= B * mb &&
-                    t->size(1) == k_cache.size(1) && t->size(2) == 16 && t->size(3) == k_cache.size(3) &&
-                    t->device() == k_cache.device(),
-                "b200.kv_dequant_pages_int8: bf16 outputs [>= B * max_blocks, Hkv, 16, D]");
   c10::cuda::CUDAGuard g(k_cache.device());
+  const auto opt = k_cache.options().dtype(at::kBFloat16);
+  Tensor k_out = at::empty({B * mb, k_cache.size(1), 16, k_cache.size(3)}, opt);
+  Tensor v_out = at::empty({B * mb, k_cache.size(1), 16, k_cache.size(3)}, opt);
+  Tensor table_out = at::empty({B, mb}, block_tables.options());
   b200::KvInt8DequantArgs a{};
   a.k_cache = k_cache.data_ptr<int8_t>();
   a.v_cache = v_cache.data_ptr<int8_t>();
@@ -696,6 +695,7 @@ void kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v_cache, const T
   a.ctx_lens = ctx_lens.data_ptr<int32_t>();
   a.k_out = static_cast<__nv_bfloat16*>(k_out.data_ptr());
   a.v_out = static_cast<__nv_bfloat16*>(v_out.data_ptr());
+  a.table_out = table_out.data_ptr<int32_t>();
   a.num_blocks = k_cache.size(0);
   a.B = (int)B;
   a.max_blocks = (int)mb;
@@ -704,19 +704,22 @@ void kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v_cache, const T
   a.status = status.data_ptr<int>();
   b200::kv_int8_dequant_launch(a, cur_stream(k_cache));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {k_out, v_out, table_out};
 }
 
-// Decode and short multi-token attention over int8 pages; returns the number of launches.
-int64_t paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
-                             const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
-                             const optional<Tensor>& cu_q, int64_t max_q_len, double scale,
-                             const optional<Tensor>& sinks, int64_t window, double softcap, Tensor& out,
-                             Tensor& status) {
+// Decode and short multi-token attention over int8 pages, into `out_opt` or a new tensor (2 launches).
+Tensor paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
+                            const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
+                            const optional<Tensor>& cu_q, int64_t max_q_len, double scale,
+                            const optional<Tensor>& sinks, int64_t window, double softcap,
+                            const optional<Tensor>& out_opt, Tensor& status) {
   check_int8_cache("paged_attention_int8", k_cache, v_cache, k_scale, v_scale);
   check_int8_tables("paged_attention_int8", k_cache, block_tables, ctx_lens);
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.is_contiguous() &&
                   q.size(2) == k_cache.size(3) && q.device() == k_cache.device(),
               "b200.paged_attention_int8: q bf16 [T, Hq, D], contiguous, on the caches' device");
+  c10::cuda::CUDAGuard g(q.device());
+  Tensor out = out_opt.has_value() && out_opt->defined() ? *out_opt : at::empty_like(q);
   TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.sizes() == q.sizes() &&
                   out.device() == q.device(),
               "b200.paged_attention_int8: out like q");
@@ -738,8 +741,7 @@ int64_t paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tenso
     TORCH_CHECK(sinks->scalar_type() == at::kFloat && sinks->numel() == Hq && sinks->is_contiguous() &&
                     sinks->device() == q.device(),
                 "b200.paged_attention_int8: sinks f32 [Hq]");
-  if (B == 0 || T == 0 || max_q_len == 0) return 0;
-  c10::cuda::CUDAGuard g(q.device());
+  if (B == 0 || T == 0 || max_q_len == 0) return out;
   b200::PagedInt8Args a{};
   a.q = static_cast<const __nv_bfloat16*>(q.data_ptr());
   a.k_cache = k_cache.data_ptr<int8_t>();
@@ -771,7 +773,7 @@ int64_t paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tenso
   a.ws = ws.data_ptr<float>();
   b200::paged_int8_launch(a, cur_stream(q));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return 2;
+  return out;
 }
 
 void kv_copy_blocks(const std::vector<Tensor>& src, const std::vector<Tensor>& dst, const Tensor& src_ids,
@@ -815,8 +817,9 @@ void kv_copy_blocks(const std::vector<Tensor>& src, const std::vector<Tensor>& d
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-void verify_drafts(const Tensor& logits, const Tensor& cu_rows, const Tensor& drafts, const optional<Tensor>& probs,
-                   const Tensor& temperature, const Tensor& uniforms, Tensor& tokens, Tensor& accepted) {
+std::vector<Tensor> verify_drafts(const Tensor& logits, const Tensor& cu_rows, const Tensor& drafts,
+                                  const optional<Tensor>& probs, const Tensor& temperature, const Tensor& uniforms,
+                                  int64_t max_drafts) {
   check_cuda(logits, "logits");
   const auto dev = logits.device();
   TORCH_CHECK(logits.scalar_type() == at::kFloat && logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
@@ -833,17 +836,16 @@ void verify_drafts(const Tensor& logits, const Tensor& cu_rows, const Tensor& dr
                   uniforms.scalar_type() == at::kFloat && uniforms.numel() == R && uniforms.is_contiguous() &&
                   uniforms.device() == dev,
               "b200.verify_drafts: temperature f32 [B], uniforms f32 [R]");
-  TORCH_CHECK(tokens.scalar_type() == at::kInt && tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) >= 1 &&
-                  tokens.is_contiguous() && tokens.device() == dev && accepted.scalar_type() == at::kInt &&
-                  accepted.numel() == B && accepted.is_contiguous() && accepted.device() == dev,
-              "b200.verify_drafts: tokens int32 [B, max_drafts + 1], accepted int32 [B]");
+  TORCH_CHECK(max_drafts >= 0 && max_drafts <= 65535, "b200.verify_drafts: 0 <= max_drafts <= 65535");
   const bool has_q = probs.has_value() && probs->defined();
   if (has_q)
     TORCH_CHECK(probs->scalar_type() == at::kFloat && probs->dim() == 2 && probs->size(0) == R - B &&
                     probs->size(1) == V && (V <= 1 || probs->stride(1) == 1) && probs->device() == dev,
                 "b200.verify_drafts: draft_probs f32 [R - B, V], rows contiguous");
-  if (B == 0) return;
   c10::cuda::CUDAGuard g(dev);
+  Tensor tokens = at::empty({B, max_drafts + 1}, cu_rows.options());
+  Tensor accepted = at::empty({B}, cu_rows.options());
+  if (B == 0) return {tokens, accepted};
   b200::VerifyArgs a{};
   a.logits = logits.data_ptr<float>();
   a.ld = logits.stride(0);
@@ -859,7 +861,7 @@ void verify_drafts(const Tensor& logits, const Tensor& cu_rows, const Tensor& dr
   a.ND = R - B;
   a.B = (int)B;
   a.V = (int)V;
-  a.max_drafts = (int)tokens.size(1) - 1;
+  a.max_drafts = (int)max_drafts;
   a.chunks = b200::verify_chunks(a.V);
   // sums of 8 bytes, maxima and indexes of 4: one workspace of this call
   const int64_t n = R * a.chunks;
@@ -869,6 +871,7 @@ void verify_drafts(const Tensor& logits, const Tensor& cu_rows, const Tensor& dr
   a.part_arg = reinterpret_cast<int32_t*>(a.part_max + n);
   b200::verify_drafts_launch(a, cur_stream(logits));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {tokens, accepted};
 }
 
 void argmax(const Tensor& logits, Tensor& out) {

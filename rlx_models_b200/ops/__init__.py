@@ -347,14 +347,9 @@ def kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_
     caches, whose block table is returned with them. Pages at or past
     ceil(ctx_lens[b] / 16) stay uninitialised (the first one of an empty
     sequence is zero)."""
-    B, mb = block_tables.shape
-    shape = (B * mb,) + tuple(k_cache.shape[1:])
-    kb = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
-    vb = torch.empty(shape, dtype=torch.bfloat16, device=k_cache.device)
     _count(1)
-    ext().kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, kb, vb,
-                                scratch(k_cache.device).status)
-    return kb, vb, torch.arange(B * mb, dtype=torch.int32, device=k_cache.device).view(B, mb)
+    return tuple(ext().kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens,
+                                             scratch(k_cache.device).status))
 
 
 INT8_DIRECT_ROWS = 64  # query rows per KV head up to which attention reads the int8 pages directly
@@ -378,18 +373,15 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     are; longer chunks are bound by their products and go through bf16 copies of
     the pages to ``prefill_attention``, whose tcgen05 products outweigh the
     copies (unless its tiles do not take the group size)."""
-    if out is None:
-        out = torch.empty_like(q)
-    Hq, Hkv = q.shape[1], k_cache.shape[1]
-    if (cu_q is not None and max_q_len * Hq > INT8_DIRECT_ROWS * Hkv and 128 * Hkv % Hq == 0
-            and block_tables.shape[1] > 0):
+    if (cu_q is not None and max_q_len * q.shape[1] > INT8_DIRECT_ROWS * k_cache.shape[1]
+            and 128 * k_cache.shape[1] % q.shape[1] == 0 and block_tables.shape[1] > 0):
         kb, vb, tables = kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens)
         return prefill_attention(q, kb, vb, tables, ctx_lens, cu_q, max_q_len, scale=scale, sinks=sinks,
                                  window=window, out=out, softcap=softcap)
-    _count(ext().paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q,
+    _count(2)
+    return ext().paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q,
                                       int(max_q_len), float(scale), sinks, int(window), float(softcap), out,
-                                      scratch(q.device).status))
-    return out
+                                      scratch(q.device).status)
 
 
 def _block_ids(ids, device) -> torch.Tensor:
@@ -443,12 +435,8 @@ def verify_drafts(logits: torch.Tensor, cu_rows: torch.Tensor, drafts: torch.Ten
     Returns tokens int32 [B, max_drafts + 1] (accepted drafts, the new token,
     then -1) and the number of accepted drafts int32 [B]. All decisions are made
     in 64 bits."""
-    B = temperature.numel()
-    tokens = torch.empty(B, int(max_drafts) + 1, dtype=torch.int32, device=logits.device)
-    accepted = torch.empty(B, dtype=torch.int32, device=logits.device)
     _count(2)
-    ext().verify_drafts(logits, cu_rows, drafts, draft_probs, temperature, uniforms, tokens, accepted)
-    return tokens, accepted
+    return tuple(ext().verify_drafts(logits, cu_rows, drafts, draft_probs, temperature, uniforms, int(max_drafts)))
 
 
 def argmax(logits: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
