@@ -37,7 +37,7 @@ constexpr int kMinExp = -100;  // smallest scale 2^-100: an all-zero block still
 // ---------------------------------------------------------------------------
 // store
 // ---------------------------------------------------------------------------
-constexpr int kStoreWarps = 8;
+constexpr int kStoreWarps = 4;
 
 // One warp per (run of adjacent tokens of one block, KV head, K or V). Lane l
 // owns 16 columns of the rows l / (D / 16) + i * (512 / D): 16-byte code loads
@@ -45,7 +45,7 @@ constexpr int kStoreWarps = 8;
 // kernel moves 3 bytes per element and is bound by launch and load latency for
 // a decode step, by HBM for a prefill.
 template <int D>
-__global__ void __launch_bounds__(kStoreWarps * 32) store_kernel(KvInt8StoreArgs a) {
+__global__ void __launch_bounds__(kStoreWarps * 32, 6) store_kernel(KvInt8StoreArgs a) {
   pdl_wait();
   pdl_trigger();
   constexpr int CPR = D / 16;       // 16-column chunks per row
@@ -81,23 +81,27 @@ __global__ void __launch_bounds__(kStoreWarps * 32) store_kernel(KvInt8StoreArgs
     }
     const int64_t page = blk * a.Hkv + h;
     const float old = scales[page];  // (asked for early; used when the block is not new)
-    // lane o < 16: newest token of the run written at offset o (-1: none)
-    int64_t src = -1;
+    // lane o < 16: newest token of the run written at offset o, from t0 (-1: none)
+    int src = -1;
     int64_t slot = __shfl_down_sync(0xffffffffu, near, at);
     int span = 32 - at;  // lanes with a slot of this piece of the run
-    for (int64_t base = t0 + at;;) {
+    for (int base = at;;) {
       const unsigned in = __ballot_sync(0xffffffffu, lane < span && slot >= 0 && (slot >> 4) == blk);
       const int len = in == 0xffffffffu ? 32 : __ffs(~in) - 1;  // tokens of the run in this piece
-      const int off = lane < len ? (int)(slot & 15) : 16 + lane;
-      const unsigned same = __match_any_sync(0xffffffffu, off);  // tokens of one offset: the last one counts
-      for (unsigned todo = __ballot_sync(0xffffffffu, off < 16 && (same >> lane) == 1u); todo != 0; todo &= todo - 1) {
-        const int from = __ffs(todo) - 1;
-        if (lane == __shfl_sync(0xffffffffu, off, from)) src = base + from;
+      const int off = lane < len ? (int)(slot & 15) : 16 + lane, off0 = __shfl_sync(0xffffffffu, off, 0);
+      if (__all_sync(0xffffffffu, lane >= len || off == off0 + lane)) {  // one behind the other
+        if (lane >= off0 && lane < off0 + len) src = base + lane - off0;
+      } else {
+        const unsigned same = __match_any_sync(0xffffffffu, off);  // tokens of one offset: the last one counts
+        for (unsigned todo = __ballot_sync(0xffffffffu, off < 16 && (same >> lane) == 1u); todo != 0; todo &= todo - 1) {
+          const int from = __ffs(todo) - 1;
+          if (lane == __shfl_sync(0xffffffffu, off, from)) src = base + from;
+        }
       }
       if (len < span) break;
       base += span;
       span = 32;
-      slot = base + lane < a.T ? a.slots[base + lane] : -1;
+      slot = t0 + base + lane < a.T ? a.slots[t0 + base + lane] : -1;
     }
     const bool fresh = __shfl_sync(0xffffffffu, src, 0) >= 0;
     const int c = (lane % CPR) * 16;
@@ -106,11 +110,11 @@ __global__ void __launch_bounds__(kStoreWarps * 32) store_kernel(KvInt8StoreArgs
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = lane / CPR + i * RPW;
-      const int64_t st = __shfl_sync(0xffffffffu, src, r);
+      const int st = __shfl_sync(0xffffffffu, src, r);
       given[i] = st >= 0;
       lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
       if (given[i]) {
-        const uint4* p = reinterpret_cast<const uint4*>(x + st * xt + h * xh + c);
+        const uint4* p = reinterpret_cast<const uint4*>(x + (t0 + st) * xt + h * xh + c);
         lo[i] = p[0];
         hi[i] = p[1];
       }
@@ -244,8 +248,9 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
       __nv_bfloat16* out = (is_v ? a.v_out : a.k_out) + dst + (is_v ? j - n : j);
       const uint2 x = widen_bf16(w[k].x, s[k]), y = widen_bf16(w[k].y, s[k]);
       const uint2 z = widen_bf16(w[k].z, s[k]), u = widen_bf16(w[k].w, s[k]);
-      reinterpret_cast<uint4*>(out)[0] = make_uint4(x.x, x.y, y.x, y.y);
-      reinterpret_cast<uint4*>(out)[1] = make_uint4(z.x, z.y, u.x, u.y);
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "r"(x.x), "r"(x.y), "r"(y.x),
+                   "r"(y.y), "r"(z.x), "r"(z.y), "r"(u.x), "r"(u.y)
+                   : "memory");
     }
   }
 }
