@@ -205,8 +205,8 @@ def main(argv=None):
         p.add_argument("--show-knobs", action="store_true", help="print the knob table at startup")
         p.add_argument("--max-model-len", type=int, default=4096)
         p.add_argument("--kv-gb", type=float, default=8.0)
-        p.add_argument("--kv-cache-dtype", default="bf16", choices=["bf16", "fp8"],
-                       help="fp8: e4m3 KV pages (half the cache bytes; the decode kernel reads them directly)")
+        p.add_argument("--kv-cache-dtype", default="bf16", choices=["bf16", "fp8", "int8"],
+                       help="half the cache bytes: fp8 (e4m3 pages, one scale per cache) or int8 (a scale per block and head)")
         if name == "run":
             p.add_argument("--prompt", default="Hello")
             p.add_argument("--ids", default=None, help="comma-separated token ids instead of --prompt")

@@ -39,6 +39,7 @@
 #include <memory>
 #include <optional>
 #include <stdexcept>
+#include <tuple>
 #include <unordered_map>
 #include <vector>
 
@@ -102,6 +103,9 @@ class BlockManager {
       free_.push_back(b);
     }
   }
+
+  // One more sequence that reads the block.
+  void share(int b) { ++ref_[b]; }
 
   // Register a full block's hash (first writer wins).
   void publish(int b, uint64_t h) {
@@ -203,6 +207,47 @@ class Scheduler {
     auto it = seqs_.find(id);
     if (it == seqs_.end() || it->second->status == FINISHED) return;
     finish(*it->second, 3);
+  }
+
+  // Branch a decoding sequence: a new one with the same tokens that reads the
+  // same full blocks. The partly filled block, which both would write, is
+  // allocated anew: the caller copies its contents. Returns (new id, block to
+  // copy, its copy), the blocks -1 when the last one is full. Tokens in flight
+  // must have been resolved.
+  std::tuple<int64_t, int32_t, int32_t> fork(int64_t id, int max_new_tokens) {
+    auto it = seqs_.find(id);
+    if (it == seqs_.end() || it->second->status != RUNNING || it->second->pending > 0 || !is_decode(*it->second))
+      throw std::invalid_argument("fork: the sequence is not decoding");
+    const Seq& p = *it->second;
+    if (p.generated() >= max_new_tokens) throw std::invalid_argument("fork: max_new_tokens is reached already");
+    if ((p.prompt_len + max_new_tokens + kBlock - 1) / kBlock > max_blocks_per_seq_)
+      throw std::invalid_argument("request longer than the model context");
+    if ((int)running_.size() >= max_num_seqs_) throw std::runtime_error("fork: max_num_seqs sequences are running");
+    const int full = p.num_computed / kBlock;
+    int32_t src = -1, dst = -1;
+    if (p.num_computed % kBlock != 0) {
+      src = p.blocks[full];
+      dst = bm_.allocate();
+      if (dst < 0) throw std::runtime_error("fork: no free KV block");
+    }
+    auto s = std::make_unique<Seq>();
+    s->id = next_id_++;
+    s->tokens = p.tokens;
+    s->prompt_len = p.prompt_len;
+    s->num_computed = p.num_computed;
+    s->max_new_tokens = max_new_tokens;
+    s->ignore_eos = p.ignore_eos;
+    s->stop_ids = p.stop_ids;
+    s->blocks.assign(p.blocks.begin(), p.blocks.begin() + full);
+    for (int b : s->blocks) bm_.share(b);
+    if (dst >= 0) s->blocks.push_back(dst);
+    s->hashes.assign(p.hashes.begin(), p.hashes.begin() + std::min((size_t)full, p.hashes.size()));
+    s->status = RUNNING;
+    s->num_cached_prompt = p.num_cached_prompt;
+    const int64_t child = s->id;
+    seqs_[child] = std::move(s);
+    running_.push_back(child);
+    return {child, src, dst};
   }
 
   bool has_work() const { return !waiting_.empty() || !running_.empty(); }
@@ -577,6 +622,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("add_request", &Scheduler::add_request, py::arg("prompt"), py::arg("max_new_tokens"),
            py::arg("ignore_eos") = false, py::arg("stop_ids") = std::vector<int32_t>{})
       .def("abort", &Scheduler::abort)
+      .def("fork", &Scheduler::fork, py::arg("seq_id"), py::arg("max_new_tokens"))
       .def("has_work", &Scheduler::has_work)
       .def("num_waiting", &Scheduler::num_waiting)
       .def("num_running", &Scheduler::num_running)

@@ -174,25 +174,32 @@ class DecoderLM:
         """Long-context decode over a bounded set of retrieved KV blocks
         (runtime/kv_retrieval.py); kw: topk_blocks, window_blocks, sink_blocks."""
         from ..runtime.kv_retrieval import KVRetrieval
+        if self.kv_dtype != torch.bfloat16:
+            raise NotImplementedError("KV retrieval reads bf16 pages")
         if any(L.window for L in self.layers) or any(L.sinks is not None for L in self.layers):
             raise NotImplementedError("KV retrieval is for full-attention layers without sinks")
         self.retrieval = KVRetrieval(self.cfg.num_hidden_layers, num_blocks, self.hkv, self.D, self.device, **kw)
 
-    kv_dtype = torch.bfloat16       # or torch.float8_e4m3fn (set_kv_cache_dtype)
+    kv_dtype = torch.bfloat16       # or torch.float8_e4m3fn, torch.int8 (set_kv_cache_dtype)
     kv_scales = (1.0, 1.0)
 
     def set_kv_cache_dtype(self, dtype: str, scales: tuple = (1.0, 1.0)) -> None:
-        """"bf16" or "fp8" (e4m3 pages holding value / scale; scales (k, v))."""
-        if dtype not in ("bf16", "fp8"):
-            raise ValueError(f"kv cache dtype {dtype!r}: 'bf16' or 'fp8'")
-        if dtype == "fp8" and getattr(self, "retrieval", None) is not None:
+        """"bf16", "fp8" (e4m3 pages holding value / scale; scales (k, v)) or "int8"
+        (codes with a scale of their own for each block and KV head)."""
+        if dtype not in ("bf16", "fp8", "int8"):
+            raise ValueError(f"kv cache dtype {dtype!r}: 'bf16', 'fp8' or 'int8'")
+        if dtype != "bf16" and getattr(self, "retrieval", None) is not None:
             raise NotImplementedError("KV retrieval reads bf16 pages")
-        self.kv_dtype = torch.float8_e4m3fn if dtype == "fp8" else torch.bfloat16
+        if dtype == "int8" and (self.D not in (64, 128) or self.hq // self.hkv > 16 or not self.cfg.causal):
+            raise NotImplementedError("int8 KV cache: causal models with head_dim 64 or 128 and at most 16 query "
+                                      "heads per KV head")
+        self.kv_dtype = {"bf16": torch.bfloat16, "fp8": torch.float8_e4m3fn, "int8": torch.int8}[dtype]
         self.kv_scales = (float(scales[0]), float(scales[1]))
 
     def kv_bytes_per_block(self) -> int:
+        int8 = self.kv_dtype == torch.int8
         return PagedKVCache.bytes_per_block(self.cfg.num_hidden_layers, self.hkv, self.D,
-                                            1 if self.kv_dtype == torch.float8_e4m3fn else 2)
+                                            2 if self.kv_dtype == torch.bfloat16 else 1, 4 if int8 else 0)
 
     def make_kv_cache(self, num_blocks: int) -> PagedKVCache:
         return PagedKVCache(self.cfg.num_hidden_layers, num_blocks, self.hkv, self.D, self.device,
@@ -212,6 +219,8 @@ class DecoderLM:
             qd, kd = self.hq * self.D, self.hkv * self.D
             ops.rmsnorm(qkv[:, :qd], L.q_norm, self.cfg.rms_norm_eps, out=qkv[:, :qd])
             ops.rmsnorm(qkv[:, qd:qd + kd], L.k_norm, self.cfg.rms_norm_eps, out=qkv[:, qd:qd + kd])
+        if kc.dtype == torch.int8:
+            return self._attention_int8(i, L, qkv, L.bqkv if acc else None, full, fb, kv)
         f8 = kc.dtype == torch.float8_e4m3fn
         sc = kv.scales if f8 else (1.0, 1.0)
         q = ops.qkv_rope(qkv, num_q_heads=self.hq, num_kv_heads=self.hkv, head_dim=self.D,
@@ -239,6 +248,28 @@ class DecoderLM:
             ops.prefill_attention(q[nd:], pk, pv, ptab, fb.pre_ctx_lens, fb.pre_cu_q,
                                   fb.pre_max_q, scale=self.scale, sinks=L.sinks, window=L.window, out=o[nd:],
                                   softcap=self.cfg.attn_softcap, causal=self.cfg.causal)
+        return o.view(T, self.hq * self.D)
+
+    def _attention_int8(self, i: int, L: LayerWeights, qkv: torch.Tensor, bias, full: bool, fb: ForwardBatch,
+                        kv: PagedKVCache):
+        """Attention over an int8 cache: K / V rows first (a block's scale depends on all of them), then the store,
+        then decode rows and prefill chunks over the pages."""
+        T, nd = qkv.shape[0], fb.num_decode
+        k = torch.empty(T, self.hkv, self.D, dtype=torch.bfloat16, device=qkv.device)
+        v = torch.empty_like(k)
+        q = ops.qkv_rope(qkv, num_q_heads=self.hq, num_kv_heads=self.hkv, head_dim=self.D, positions=fb.positions,
+                         inv_freq=L.inv_freq, rope_scale=L.rope_mult, rot_dim=self.cfg.rotary_dim,
+                         q_norm=None if full else L.q_norm, k_norm=None if full else L.k_norm,
+                         eps=self.cfg.rms_norm_eps, k_out=k, v_out=v, bias=bias)
+        cache = kv.int8_layer(i)
+        ops.kv_store_int8(k, v, fb.slots, *cache)
+        o = torch.empty_like(q)
+        kw = dict(scale=self.scale, sinks=L.sinks, window=L.window, softcap=self.cfg.attn_softcap)
+        if nd > 0:
+            ops.paged_attention_int8(q[:nd], *cache, fb.dec_block_tables, fb.dec_ctx_lens, out=o[:nd], **kw)
+        if T > nd:
+            ops.paged_attention_int8(q[nd:], *cache, fb.pre_block_tables, fb.pre_ctx_lens, cu_q=fb.pre_cu_q,
+                                     max_q_len=fb.pre_max_q, out=o[nd:], **kw)
         return o.view(T, self.hq * self.D)
 
     def _layer(self, i: int, L: LayerWeights, x: torch.Tensor, h: torch.Tensor, fb: ForwardBatch, kv, comm,

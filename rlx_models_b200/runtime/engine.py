@@ -107,8 +107,9 @@ class EngineConfig:
     # long-context decode over retrieved KV blocks, e.g. {"topk_blocks": 64,
     # "window_blocks": 16, "sink_blocks": 1} (runtime/kv_retrieval.py); None = full attention
     kv_retrieval: dict | None = None
-    # "bf16", or "fp8": float8 e4m3 pages holding value / scale with scales (k, v) (the
-    # decode kernel reads them directly; prefill reads bf16 copies of its pages)
+    # "bf16"; "fp8": float8 e4m3 pages holding value / scale with scales (k, v) (the
+    # decode kernel reads them directly; prefill reads bf16 copies of its pages); "int8":
+    # codes with a scale for each block and KV head, no scales to choose
     kv_cache_dtype: str = "bf16"
     kv_cache_scales: tuple = (1.0, 1.0)
     # schedule / launch step n+1 before step n's tokens come back (see module docstring)
@@ -230,6 +231,7 @@ class LLMEngine:
         self._n_host_rows = 0   # active requests that need the host between steps (penalties, processors)
         self._n_mm = 0          # active requests with input embeddings (images)
         self._inflight = None
+        self._early: list[RequestOutput] = []  # finished while fork() drained the step in flight
         self.graphs: dict[int, tuple] = {}
         self._graph_pool = None
         self.stats = dict(steps=0, graph_steps=0, eager_steps=0, tokens=0, h2d_bytes=0, d2h_bytes=0,
@@ -287,6 +289,38 @@ class LLMEngine:
         self.sched.abort(sid)
         self._retire(sid)
 
+    def fork(self, sid: int, params: SamplingParams | None = None) -> int:
+        """Branch a running request that has generated at least one token: a new
+        request with the same prompt and the same output so far, which goes on by
+        itself under ``params`` (default: the parent's; ``max_new_tokens`` counts
+        from the prompt). Both read the same full KV blocks; the partly filled
+        one is copied on the device. Returns the new request's id."""
+        if self.stateful or self.cfg.kv_retrieval or hasattr(self.model, "share_tokens") \
+                or not hasattr(self.kv, "copy_blocks"):
+            raise NotImplementedError(f"{type(self.model).__name__}: fork needs a paged KV cache and nothing beside it")
+        if self._inflight is not None:  # its tokens have to be known
+            self._early += self._finish(self._inflight)
+            self._inflight = None
+        st = self.requests.get(sid)
+        if st is None:
+            raise ValueError(f"fork: request {sid} is not running")
+        params = params or st.params
+        if st.prompt is None and (params.repetition_penalty != 1.0 or params.dry_multiplier > 0):
+            raise ValueError("fork: the parent keeps no prompt for a repetition penalty or DRY")
+        child, src, dst = self.sched.fork(sid, int(params.max_new_tokens))
+        if src >= 0:
+            self.kv.copy_blocks([src], [dst])
+        new = dataclasses.replace(st, seq_id=child, params=params, token_times=list(st.token_times),
+                                  tokens=list(st.tokens), logprobs=list(st.logprobs), rng=None, mirostat_mu=None,
+                                  mirostat_lp2=None, out_counts=None)
+        if params.penalised or params.processed:
+            new.out_counts = dict(collections.Counter(st.tokens))
+        if new.mm is not None:
+            self._n_mm += 1
+        self.requests[child] = new
+        self._track(new, +1)
+        return child
+
     def _free_slot(self, sid: int):
         if self.stateful and sid in self.slot_of:
             self.free_slots.append(self.slot_of.pop(sid))
@@ -303,7 +337,7 @@ class LLMEngine:
         return len(ids)
 
     def has_unfinished(self) -> bool:
-        return self.sched.has_work() or self._inflight is not None
+        return self.sched.has_work() or self._inflight is not None or bool(self._early)
 
     # -- model step ------------------------------------------------------------
     def _params_rows(self, sids: list[int]) -> bool:
@@ -503,14 +537,15 @@ class LLMEngine:
         """One engine iteration. With overlapped scheduling this launches the
         next step and returns the requests finished by the previous one."""
         with nvtx("engine.step"):
+            early, self._early = self._early, []
             if self._can_overlap():
                 inf = self._launch(overlap=True)
                 outs = self._finish(self._inflight) if self._inflight is not None else []
                 self._inflight = inf
-                return outs
-            outs = []
+                return early + outs
+            outs = early
             if self._inflight is not None:  # leave overlapped mode: drain the step in flight first
-                outs = self._finish(self._inflight)
+                outs += self._finish(self._inflight)
                 self._inflight = None
             inf = self._launch(overlap=False)
             if inf is not None:

@@ -56,10 +56,8 @@ def save_prompt(engine, path: str, tokens: list[int]) -> int:
     blocks = engine.sched.prefix_blocks(tokens)
     n = len(blocks)
     kv = engine.kv
-    idx = torch.tensor(blocks, dtype=torch.long, device=kv.k.device)
-    tensors = {"k": kv.k.index_select(1, idx).cpu() if n else torch.empty(0),
-               "v": kv.v.index_select(1, idx).cpu() if n else torch.empty(0),
-               "tokens": torch.tensor(tokens[:n * BLOCK_SIZE], dtype=torch.int32)}
+    tensors = {name: t.cpu() if n else torch.empty(0) for name, t in kv.gather_blocks(blocks).items()}
+    tensors["tokens"] = torch.tensor(tokens[:n * BLOCK_SIZE], dtype=torch.int32)
     meta = {"format": FORMAT, "fingerprint": model_fingerprint(engine.model, kv), "blocks": str(n)}
     save_file(tensors, path, metadata=meta)
     return n * BLOCK_SIZE
@@ -79,13 +77,10 @@ def load_prompt(engine, path: str) -> int:
         tokens = f.get("tokens").tolist()
         blocks = engine.sched.import_prefix(tokens)
         kv = engine.kv
-        k, v = f.get("k").clone(), f.get("v").clone()  # copies: the file's mapping closes below
         fill = [(i, b) for i, b in enumerate(blocks) if b >= 0]
         if fill:
-            src = torch.tensor([i for i, _ in fill], dtype=torch.long)
-            dst = torch.tensor([b for _, b in fill], dtype=torch.long, device=kv.k.device)
-            kv.k.index_copy_(1, dst, k.index_select(1, src).to(kv.k.device))
-            kv.v.index_copy_(1, dst, v.index_select(1, src).to(kv.v.device))
+            saved = {name: f.get(name).clone() for name in kv.tensors()}  # copies: the file's mapping closes below
+            kv.scatter_blocks(saved, [i for i, _ in fill], [b for _, b in fill])
         return len(blocks) * BLOCK_SIZE
     finally:
         f.close()

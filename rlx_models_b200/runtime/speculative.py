@@ -14,6 +14,12 @@ Proposers:
   * prompt lookup (no model): the tokens that followed the most recent earlier
     occurrence of the current n-gram suffix (n = ngram .. 1).
 
+Sampled generation (``temperature`` > 0) keeps the target's distribution: a
+draft model's tokens are drawn from its own softmax and accepted with
+probability min(1, p / q), the first refused position draws from max(p - q, 0)
+(``ops.verify_drafts``, decided on the device in 64 bits from given uniform
+numbers); looked-up tokens and a learned head's count as certain drafts (q = 1).
+
 KV caches are positional (slot = position under an identity block table), so
 rolling back after a rejection is just moving the position: stale entries past
 it are overwritten by the next writes.
@@ -112,6 +118,7 @@ class SpeculativeDecoder:
         self.head, self.head_window = draft_head, head_window
         self.k, self.ngram = k, ngram
         self.stats = SpecStats()
+        self._gen, self._temperature, self._draft_probs = None, 0.0, []
 
     def _propose_head(self, seq: list[int], k: int) -> list[int]:
         """Learned draft head over the target's features of the last positions."""
@@ -126,11 +133,39 @@ class SpeculativeDecoder:
         # catch up: feed every accepted token the draft has not seen (the last one included)
         pending = seq[d.pos:]
         lg = d.run(pending, d.pos)
-        props = [int(lg[-1].argmax())]
+        self._draft_probs = []
+        props = [self._pick(lg[-1])]
         for _ in range(k - 1):
             lg = d.run([props[-1]], d.pos)
-            props.append(int(lg[-1].argmax()))
+            props.append(self._pick(lg[-1]))
         return props
+
+    def _pick(self, logits: torch.Tensor) -> int:
+        """The draft model's token: its argmax, or a draw whose distribution is kept for the verification."""
+        if self._gen is None:
+            return int(logits.argmax())
+        q = torch.softmax(logits.float() / self._temperature, -1)
+        self._draft_probs.append(q)
+        return int(torch.multinomial(q, 1, generator=self._gen))
+
+    def _verify(self, props: list[int], lv: torch.Tensor) -> tuple[list[int], int]:
+        """Target logits [len(props) + 1, V] -> (accepted proposals and the token behind them, number accepted)."""
+        if self._gen is None:
+            tgt = lv.argmax(-1).tolist()
+            n_acc = 0
+            while n_acc < len(props) and props[n_acc] == tgt[n_acc]:
+                n_acc += 1
+            return props[:n_acc] + [tgt[n_acc]], n_acc
+        from .. import ops
+        dev, n = lv.device, len(props)
+        q = torch.stack(self._draft_probs[:n]) if self.draft is not None and self.head is None and n else None
+        tokens, acc = ops.verify_drafts(
+            lv.float(), torch.tensor([0, n + 1], dtype=torch.int32, device=dev),
+            torch.tensor(props, dtype=torch.int32, device=dev), q,
+            torch.full((1,), self._temperature, device=dev), torch.rand(n + 1, generator=self._gen, device=dev),
+            max_drafts=n)
+        n_acc = int(acc[0])
+        return tokens[0, :n_acc + 1].tolist(), n_acc
 
     def _propose_lookup(self, seq: list[int], k: int) -> list[int]:
         for n in range(min(self.ngram, len(seq) - 1), 0, -1):
@@ -144,14 +179,20 @@ class SpeculativeDecoder:
 
     # -- generation --------------------------------------------------------------
     @torch.no_grad()
-    def generate(self, prompt: list[int], max_new_tokens: int, eos_token_id: int | None = None) -> list[int]:
+    def generate(self, prompt: list[int], max_new_tokens: int, eos_token_id: int | None = None,
+                 temperature: float = 0.0, seed: int = 0) -> list[int]:
+        """Greedy, or with ``temperature`` > 0 a draw from the target's softmax(logits / temperature) that
+        ``seed`` repeats."""
         t = self.target
         t.pos = 0
+        self._gen, self._temperature = None, float(temperature)
+        if temperature > 0:
+            self._gen = torch.Generator(device=t.model.device).manual_seed(seed)
         if self.draft is not None:
             self.draft.pos = 0
         keep = self.head is not None
         lg = t.run(list(prompt), 0, keep)
-        seq = list(prompt) + [int(lg[-1].argmax())]
+        seq = list(prompt) + self._verify([], lg[-1:])[0]
         out = [seq[-1]]
         while len(out) < max_new_tokens and (eos_token_id is None or out[-1] != eos_token_id):
             k = min(self.k, max_new_tokens - len(out))
@@ -165,14 +206,10 @@ class SpeculativeDecoder:
             start = len(seq) - 1
             snap = _snapshot(t.kv) if self.stateful and props else None
             lv = t.run([seq[-1]] + props, start, keep)
-            tgt = lv.argmax(-1).tolist()
-            n_acc = 0
-            while n_acc < len(props) and props[n_acc] == tgt[n_acc]:
-                n_acc += 1
+            new, n_acc = self._verify(props, lv)
             if snap is not None and n_acc < len(props):
                 _restore(t.kv, snap)
                 t.run([seq[-1]] + props[:n_acc], start, keep)
-            new = props[:n_acc] + [tgt[n_acc]]
             self.stats.target_passes += 1
             self.stats.proposed += len(props)
             self.stats.accepted += n_acc
