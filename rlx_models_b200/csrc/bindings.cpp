@@ -707,12 +707,14 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   return {k_out, v_out, table_out};
 }
 
-// Decode and short multi-token attention over int8 pages, into `out_opt` or a new tensor (2 launches).
-Tensor paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
-                            const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
-                            const optional<Tensor>& cu_q, int64_t max_q_len, double scale,
-                            const optional<Tensor>& sinks, int64_t window, double softcap,
-                            const optional<Tensor>& out_opt, Tensor& status) {
+// Decode and short multi-token attention over int8 pages, into `out_opt` or a new tensor; and
+// the number of launches.
+std::tuple<Tensor, int64_t> paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                                                 const Tensor& k_scale, const Tensor& v_scale,
+                                                 const Tensor& block_tables, const Tensor& ctx_lens,
+                                                 const optional<Tensor>& cu_q, int64_t max_q_len, double scale,
+                                                 const optional<Tensor>& sinks, int64_t window, double softcap,
+                                                 const optional<Tensor>& out_opt, Tensor& status) {
   check_int8_cache("paged_attention_int8", k_cache, v_cache, k_scale, v_scale);
   check_int8_tables("paged_attention_int8", k_cache, block_tables, ctx_lens);
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.is_contiguous() &&
@@ -741,7 +743,7 @@ Tensor paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor
     TORCH_CHECK(sinks->scalar_type() == at::kFloat && sinks->numel() == Hq && sinks->is_contiguous() &&
                     sinks->device() == q.device(),
                 "b200.paged_attention_int8: sinks f32 [Hq]");
-  if (B == 0 || T == 0 || max_q_len == 0) return out;
+  if (B == 0 || T == 0 || max_q_len == 0) return {out, 0};
   b200::PagedInt8Args a{};
   a.q = static_cast<const __nv_bfloat16*>(q.data_ptr());
   a.k_cache = k_cache.data_ptr<int8_t>();
@@ -768,12 +770,13 @@ Tensor paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor
   a.status = status.data_ptr<int>();
   a.device = q.get_device();
   // a workspace of this call: the allocator orders its reuse by stream, and a captured graph keeps its own
-  Tensor ws = at::empty({b200::paged_int8_ws_floats(a.device, a.B, a.Hkv, a.G, a.D, a.max_q_len, a.max_blocks)},
+  Tensor ws = at::empty({b200::paged_int8_ws_floats(a.device, a.B, a.Hkv, a.G, a.D, a.max_q_len, a.max_blocks,
+                                                         a.window)},
                         q.options().dtype(at::kFloat));
   a.ws = ws.data_ptr<float>();
-  b200::paged_int8_launch(a, cur_stream(q));
+  const int n = b200::paged_int8_launch(a, cur_stream(q));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return out;
+  return {out, n};
 }
 
 void kv_copy_blocks(const std::vector<Tensor>& src, const std::vector<Tensor>& dst, const Tensor& src_ids,

@@ -381,14 +381,15 @@ struct PagedInt8Args {
   const float* sinks;       // [Hq] or null
   float* ws;                // paged_int8_ws_floats() floats: two parts per warp, then ws_pre
   int32_t* ws_pre = nullptr;  // [B + 1] (set by the launcher)
+  int whole = 0;              // warps take whole segments (set by the launcher)
   int64_t num_blocks;
   int B, T, Hq, Hkv, G, D, max_blocks, max_q_len, window;
   float scale, softcap;
   int* status;
   int device;
 };
-int64_t paged_int8_ws_floats(int device, int B, int Hkv, int G, int D, int max_q_len, int max_blocks);
-void paged_int8_launch(const PagedInt8Args& a, cudaStream_t st);
+int64_t paged_int8_ws_floats(int device, int B, int Hkv, int G, int D, int max_q_len, int max_blocks, int window);
+int paged_int8_launch(const PagedInt8Args& a, cudaStream_t st);  // returns #launches
 
 // Blocks of a cache copied over all layers, up to four tensors in one launch: see attention/kv_copy.cu.
 struct KvCopyArgs {

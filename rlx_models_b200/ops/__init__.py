@@ -378,10 +378,11 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         kb, vb, tables = kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens)
         return prefill_attention(q, kb, vb, tables, ctx_lens, cu_q, max_q_len, scale=scale, sinks=sinks,
                                  window=window, out=out, softcap=softcap)
-    _count(2)
-    return ext().paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q,
-                                      int(max_q_len), float(scale), sinks, int(window), float(softcap), out,
-                                      scratch(q.device).status)
+    out, n = ext().paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q,
+                                        int(max_q_len), float(scale), sinks, int(window), float(softcap), out,
+                                        scratch(q.device).status)
+    _count(n)
+    return out
 
 
 def _block_ids(ids, device) -> torch.Tensor:
