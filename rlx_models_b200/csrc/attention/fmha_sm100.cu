@@ -32,6 +32,7 @@
 #include <algorithm>
 #include <cstdlib>
 #include <stdexcept>
+#include <type_traits>
 
 #include "../common/b200.cuh"
 #include "../common/launch.h"
@@ -159,6 +160,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t* st = KVs + s * kStage;
         const int page0 = (k_begin >> 4) + j * (kBN / 16);
         mbar_arrive_expect_tx(&k_full[s], kKV);
+        if (a.kv_contig) {  // the tile's 8 pages are one box (pages past the context hold zeros and are masked)
+          mbar_arrive_expect_tx(&v_full[s], kKV);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            tma_load_4d(st + h * kHalf, &tmK, &k_full[s], h * 64, 0, hkv, b * a.max_blocks + page0);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            tma_load_4d(st + kKV + h * kHalf, &tmV, &v_full[s], h * 64, 0, hkv, b * a.max_blocks + page0);
+          if (++s == kNST) {
+            s = 0;
+            ph ^= 1;
+          }
+          continue;
+        }
         for (int pg = 0; pg < kBN / 16; ++pg) {
           const int blk = btab[min(page0 + pg, max_page - 1)];  // pages past the context are masked
 #pragma unroll
@@ -267,15 +282,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         lo = max(0, kmin - key0);
         hi = min(kBN, kmax - key0);
       }
-      float mx = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < kBN / 32; ++c) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(sb + c * 32, v);
-        tmem_wait_ld();
+      // the row's scores, read once; most tiles lie inside every row's range and need no masks
+      uint32_t sv[kBN / 32][32];
 #pragma unroll
-        for (int t = 0; t < 32; ++t)
-          if (c * 32 + t >= lo && c * 32 + t < hi) mx = fmaxf(mx, __uint_as_float(v[t]));
+      for (int c = 0; c < kBN / 32; ++c) tmem_ld_32x32b_x32(sb + c * 32, sv[c]);
+      tmem_wait_ld();
+      const bool inside = __all_sync(0xffffffffu, lo == 0 && hi == kBN);
+      float mx = -INFINITY;
+      if (inside) {
+#pragma unroll
+        for (int c = 0; c < kBN / 32; ++c)
+#pragma unroll
+          for (int t = 0; t < 32; ++t) mx = fmaxf(mx, __uint_as_float(sv[c][t]));
+      } else {
+#pragma unroll
+        for (int c = 0; c < kBN / 32; ++c)
+#pragma unroll
+          for (int t = 0; t < 32; ++t)
+            if (c * 32 + t >= lo && c * 32 + t < hi) mx = fmaxf(mx, __uint_as_float(sv[c][t]));
       }
       const float m_tile = mx * sl2;
       const bool grow = m_tile > m_used + kRescale;  // this row's max moved by more than 2^8
@@ -302,22 +326,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= f;
       }
       if (grow) m_used = m_tile;
-#pragma unroll 1
-      for (int c = 0; c < kBN / 32; ++c) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(sb + c * 32, v);
-        tmem_wait_ld();
-        uint32_t pk[16];
+      auto weights = [&](auto masked) {
 #pragma unroll
-        for (int t = 0; t < 32; t += 2) {
-          const int k0 = c * 32 + t;
-          const float p0 = (k0 >= lo && k0 < hi) ? ex2(__uint_as_float(v[t]) * sl2 - m_used) : 0.f;
-          const float p1 = (k0 + 1 >= lo && k0 + 1 < hi) ? ex2(__uint_as_float(v[t + 1]) * sl2 - m_used) : 0.f;
-          l += p0 + p1;
-          pk[t / 2] = pack_bf16x2(p0, p1);
+        for (int c = 0; c < kBN / 32; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int t = 0; t < 32; t += 2) {
+            float p0 = ex2(__uint_as_float(sv[c][t]) * sl2 - m_used);
+            float p1 = ex2(__uint_as_float(sv[c][t + 1]) * sl2 - m_used);
+            if constexpr (decltype(masked)::value) {
+              const int k0 = c * 32 + t;
+              if (k0 < lo || k0 >= hi) p0 = 0.f;
+              if (k0 + 1 < lo || k0 + 1 >= hi) p1 = 0.f;
+            }
+            l += p0 + p1;
+            pk[t / 2] = pack_bf16x2(p0, p1);
+          }
+          tmem_st_32x32b_x16(sb + c * 16, pk);  // over S columns already consumed
         }
-        tmem_st_32x32b_x16(sb + c * 16, pk);  // over S columns already consumed
-      }
+      };
+      if (inside) weights(std::false_type{});
+      else weights(std::true_type{});
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -388,7 +417,10 @@ void fmha_launch(const AttnArgs& a, cudaStream_t st) {
   CUtensorMap tq = make_tmap_3d(a.q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kD, a.Hq, a.q_rows, kD,
                                 (uint64_t)a.Hq * kD, 64, G, 16);
   CUtensorMap tk, tv;
-  if (a.kv_dense) {  // [rows, Hkv, D]: one 16-row page of one head = box [16][1][64]
+  if (a.kv_contig) {  // [pages, Hkv, 16, D]: 8 pages of one head = box [8][1][16][64]
+    tk = make_tmap_4d(a.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kD, 16, a.Hkv, a.num_blocks, 64, 16, 1, 8);
+    tv = make_tmap_4d(a.v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kD, 16, a.Hkv, a.num_blocks, 64, 16, 1, 8);
+  } else if (a.kv_dense) {  // [rows, Hkv, D]: one 16-row page of one head = box [16][1][64]
     tk = make_tmap_3d(a.k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kD, a.Hkv, a.kv_rows, kD,
                       (uint64_t)a.Hkv * kD, 64, 1, 16);
     tv = make_tmap_3d(a.v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kD, a.Hkv, a.kv_rows, kD,

@@ -217,12 +217,13 @@ constexpr int kDequantThreads = 128, kDequantSteps = 4;
 __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int b = blockIdx.x / a.max_blocks, p = blockIdx.x % a.max_blocks;
-  const int id = a.tables[blockIdx.x], ctx = a.ctx_lens[b];
+  const int b = blockIdx.x / a.out_blocks, p = blockIdx.x % a.out_blocks;
+  const int id = p < a.max_blocks ? a.tables[(int64_t)b * a.max_blocks + p] : -1, ctx = a.ctx_lens[b];
   if (a.table_out != nullptr && blockIdx.y == 0 && threadIdx.x == 0) a.table_out[blockIdx.x] = blockIdx.x;
-  if (p * 16 >= ctx && p > 0) return;
-  const bool known = id >= 0 && id < a.num_blocks && ctx > 0;
-  if (!known && ctx > 0 && threadIdx.x == 0) report_error(a.status, kErrBounds, id);
+  const int pages = (ctx + 15) / 16, filled = (max(pages, 1) + a.pad - 1) / a.pad * a.pad;
+  if (p >= filled) return;
+  const bool known = p < pages && id >= 0 && id < a.num_blocks;
+  if (!known && p < pages && threadIdx.x == 0) report_error(a.status, kErrBounds, id);
   const int head = 16 * a.D, n = a.Hkv * head;
   const int64_t src = (int64_t)id * n, dst = (int64_t)blockIdx.x * n;
   const int j0 = (blockIdx.y * kDequantSteps * kDequantThreads + threadIdx.x) * 16;
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
   for (int k = 0; k < kDequantSteps; ++k) {  // K codes, then V codes
     const int j = j0 + k * kDequantThreads * 16;
     w[k] = make_uint4(0, 0, 0, 0);
-    s[k] = 0.f;  // the first page of an empty sequence, which attention may still load, and unknown pages hold zeros
+    s[k] = 0.f;  // unknown pages and those behind a context that attention may still load hold zeros
     if (known && j < 2 * n) {
       const bool is_v = j >= n;
       const int c = is_v ? j - n : j;
@@ -1014,10 +1015,10 @@ void kv_int8_store_launch(const KvInt8StoreArgs& args, int D, cudaStream_t st) {
 }
 
 void kv_int8_dequant_launch(const KvInt8DequantArgs& a, cudaStream_t st) {
-  if (a.B == 0 || a.max_blocks == 0) return;
+  if (a.B == 0 || a.out_blocks == 0) return;
   const int per_cta = kv8::kDequantThreads * kv8::kDequantSteps * 16;
   const int parts = (2 * a.Hkv * 16 * a.D + per_cta - 1) / per_cta;
-  launch_pdl(kv8::dequant_kernel, dim3((unsigned)(a.B * a.max_blocks), (unsigned)parts), dim3(kv8::kDequantThreads), 0,
+  launch_pdl(kv8::dequant_kernel, dim3((unsigned)(a.B * a.out_blocks), (unsigned)parts), dim3(kv8::kDequantThreads), 0,
              st, a);
 }
 

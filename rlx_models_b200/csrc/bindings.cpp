@@ -569,7 +569,7 @@ int64_t decode_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v
 void prefill_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_tables,
                        const Tensor& ctx_lens, const Tensor& cu_q, Tensor& out, const optional<Tensor>& sinks,
                        int64_t window, double scale, int64_t max_q_len, Tensor& status, bool causal, bool q_paged,
-                       double softcap) {
+                       double softcap, bool kv_contig) {
   c10::cuda::CUDAGuard g(q.device());
   auto a = attn_args(q, k_cache, v_cache, block_tables, ctx_lens, out, sinks, window, scale, status);
   TORCH_CHECK(!a.kv_fp8, "b200.prefill: fp8 pages are read through kv_dequant_pages (bf16 copies)");
@@ -580,6 +580,12 @@ void prefill_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_c
   a.causal = causal ? 1 : 0;
   a.q_paged = q_paged ? 1 : 0;
   a.q_rows = q.size(0);
+  if (kv_contig) {
+    TORCH_CHECK(k_cache.dim() == 4 && block_tables.size(1) % 8 == 0 &&
+                    k_cache.size(0) >= block_tables.size(0) * block_tables.size(1) && !q_paged,
+                "b200.prefill: consecutive pages need max_blocks % 8 == 0 and B * max_blocks blocks");
+    a.kv_contig = b200::fmha_supported(a) ? 1 : 0;  // (the other kernel reads the same pages through the table)
+  }
   if (k_cache.dim() == 3) {  // row-major [rows, Hkv, D] keys / values
     a.kv_dense = 1;
     a.kv_rows = k_cache.size(0);
@@ -676,16 +682,18 @@ static void check_int8_tables(const char* op, const Tensor& k_cache, const Tenso
 
 std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
                                           const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
-                                          Tensor& status) {
+                                          Tensor& status, int64_t pad) {
   check_int8_cache("kv_dequant_pages_int8", k_cache, v_cache, k_scale, v_scale);
   check_int8_tables("kv_dequant_pages_int8", k_cache, block_tables, ctx_lens);
   const int64_t B = block_tables.size(0), mb = block_tables.size(1);
-  TORCH_CHECK(B * mb <= INT32_MAX, "b200.kv_dequant_pages_int8: block_tables too large");
+  TORCH_CHECK(pad >= 1 && pad <= 64, "b200.kv_dequant_pages_int8: 1 <= pad <= 64");
+  const int64_t ob = (mb + pad - 1) / pad * pad;  // blocks of a sequence in the copies
+  TORCH_CHECK(B * ob <= INT32_MAX, "b200.kv_dequant_pages_int8: block_tables too large");
   c10::cuda::CUDAGuard g(k_cache.device());
   const auto opt = k_cache.options().dtype(at::kBFloat16);
-  Tensor k_out = at::empty({B * mb, k_cache.size(1), 16, k_cache.size(3)}, opt);
-  Tensor v_out = at::empty({B * mb, k_cache.size(1), 16, k_cache.size(3)}, opt);
-  Tensor table_out = at::empty({B, mb}, block_tables.options());
+  Tensor k_out = at::empty({B * ob, k_cache.size(1), 16, k_cache.size(3)}, opt);
+  Tensor v_out = at::empty({B * ob, k_cache.size(1), 16, k_cache.size(3)}, opt);
+  Tensor table_out = at::empty({B, ob}, block_tables.options());
   b200::KvInt8DequantArgs a{};
   a.k_cache = k_cache.data_ptr<int8_t>();
   a.v_cache = v_cache.data_ptr<int8_t>();
@@ -699,6 +707,8 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   a.num_blocks = k_cache.size(0);
   a.B = (int)B;
   a.max_blocks = (int)mb;
+  a.out_blocks = (int)ob;
+  a.pad = (int)pad;
   a.Hkv = (int)k_cache.size(1);
   a.D = (int)k_cache.size(3);
   a.status = status.data_ptr<int>();
@@ -1899,7 +1909,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prefill_attention", &prefill_attention, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("block_tables"), py::arg("ctx_lens"), py::arg("cu_q"), py::arg("out"), py::arg("sinks"),
         py::arg("window"), py::arg("scale"), py::arg("max_q_len"), py::arg("status"), py::arg("causal"),
-        py::arg("q_paged"), py::arg("softcap") = 0.0);
+        py::arg("q_paged"), py::arg("softcap") = 0.0, py::arg("kv_contig") = false);
   m.def("argmax", &argmax);
   m.def("forward_tokens", &forward_tokens);
   m.def("tp_argmax", &tp_argmax);
@@ -1914,7 +1924,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("instance_norm", &instance_norm);
   m.def("kv_dequant_pages", &kv_dequant_pages);
   m.def("kv_store_int8", &kv_store_int8);
-  m.def("kv_dequant_pages_int8", &kv_dequant_pages_int8);
+  m.def("kv_dequant_pages_int8", &kv_dequant_pages_int8, py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("block_tables"), py::arg("ctx_lens"), py::arg("status"), py::arg("pad") = 1);
   m.def("paged_attention_int8", &paged_attention_int8);
   m.def("kv_copy_blocks", &kv_copy_blocks);
   m.def("verify_drafts", &verify_drafts);

@@ -312,6 +312,8 @@ struct AttnArgs {
   int64_t q_rows = 0;        // prefill: rows of q (bounds of its TMA map)
   int kv_dense = 0;          // prefill: k/v row-major [kv_rows, Hkv, D] (pages = 16 consecutive rows)
   int64_t kv_rows = 0;
+  int kv_contig = 0;         // prefill (tcgen05 kernel): page p of sequence b is block b * max_blocks + p, max_blocks a
+                             // multiple of 8, pages between a context's end and the next multiple of 8 finite
   float* lse = nullptr;      // prefill (tcgen05 kernel, no sinks): per (row, head) log2-sum-exp2 of the
                              // scaled scores, [q_rows][Hq], for the attention backward
   float* ws;                 // decode split workspace
@@ -361,9 +363,11 @@ struct KvInt8DequantArgs {
   const int32_t* ctx_lens;  // [B]
   __nv_bfloat16* k_out;
   __nv_bfloat16* v_out;
-  int32_t* table_out;       // [B, max_blocks] or null: the copies' block table, 0, 1, 2 ...
+  int32_t* table_out;       // [B, out_blocks] or null: the copies' block table, 0, 1, 2 ...
   int64_t num_blocks;
   int B, max_blocks, Hkv, D;
+  int out_blocks;           // blocks of a sequence in the copies (>= max_blocks): page p at b * out_blocks + p
+  int pad;                  // pages from a context's end to the next multiple of this are zeros (1: none but the first)
   int* status;
 };
 void kv_int8_dequant_launch(const KvInt8DequantArgs& a, cudaStream_t st);

@@ -73,6 +73,23 @@ inline CUtensorMap make_tmap_3d(const void* base, CUtensorMapDataType dtype, int
   return m;
 }
 
+// 4-D tiled map over a contiguous [d3][d2][d1][d0] with box [b3][b2][b1][b0] and 128-byte swizzle.
+inline CUtensorMap make_tmap_4d(const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t d0, uint64_t d1,
+                                uint64_t d2, uint64_t d3, uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0) throw std::runtime_error("b200: TMA base not 16B aligned");
+  if ((d0 * elem_bytes) % 16 != 0) throw std::runtime_error("b200: TMA strides not 16B multiples");
+  CUtensorMap m;
+  cuuint64_t dims[4] = {d0, d1, d2, d3};
+  cuuint64_t strides[3] = {d0 * elem_bytes, d0 * d1 * elem_bytes, d0 * d1 * d2 * elem_bytes};
+  cuuint32_t box[4] = {b0, b1, b2, b3};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = get_encode_tiled()(&m, dtype, 4, const_cast<void*>(base), dims, strides, box, estr,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("b200: cuTensorMapEncodeTiled (4d) failed: " + std::to_string((int)r));
+  return m;
+}
+
 inline int num_sms(int device) {
   static int cache[64] = {0};
   if (device < 0 || device >= 64) device = 0;

@@ -375,9 +375,16 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     copies (unless its tiles do not take the group size)."""
     if (cu_q is not None and max_q_len * q.shape[1] > INT8_DIRECT_ROWS * k_cache.shape[1]
             and 128 * k_cache.shape[1] % q.shape[1] == 0 and block_tables.shape[1] > 0):
-        kb, vb, tables = kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens)
-        return prefill_attention(q, kb, vb, tables, ctx_lens, cu_q, max_q_len, scale=scale, sinks=sinks,
-                                 window=window, out=out, softcap=softcap)
+        # copies of a sequence lie in a row and end on a multiple of 8 pages: one box of the kernel's loads
+        status = scratch(q.device).status
+        kb, vb, tables = ext().kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens,
+                                                     status, pad=8)
+        if out is None:
+            out = torch.empty_like(q)
+        _count(2)
+        ext().prefill_attention(q, kb, vb, tables, ctx_lens, cu_q, out, sinks, int(window), float(scale),
+                                int(max_q_len), status, True, False, float(softcap), kv_contig=True)
+        return out
     out, n = ext().paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q,
                                         int(max_q_len), float(scale), sinks, int(window), float(softcap), out,
                                         scratch(q.device).status)
