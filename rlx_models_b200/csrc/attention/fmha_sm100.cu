@@ -99,7 +99,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();
   const int G = a.Hq / a.Hkv;
-  const int b = blockIdx.x / q_tiles, qt = blockIdx.x % q_tiles, hkv = blockIdx.y;
+  // last query tiles first: under a causal mask they are the longest, and the short ones fill the tail
+  const int b = blockIdx.x % a.B, qt = q_tiles - 1 - blockIdx.x / a.B, hkv = blockIdx.y;
   const int q0 = a.cu_q[b];
   const int q_len = a.cu_q[b + 1] - q0;
   const int tok0 = qt * rows_tok;
