@@ -218,7 +218,12 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
   pdl_wait();
   pdl_trigger();
   const int b = blockIdx.x / a.out_blocks, p = blockIdx.x % a.out_blocks;
-  const int id = p < a.max_blocks ? a.tables[(int64_t)b * a.max_blocks + p] : -1, ctx = a.ctx_lens[b];
+  const int id = p < a.max_blocks ? a.tables[(int64_t)b * a.max_blocks + p] : -1;
+  const int ctx = min(max(a.ctx_lens[b], 0), a.max_blocks * 16);
+  if (p == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    if (a.ctx_out != nullptr) a.ctx_out[b] = ctx;
+    if (a.ctx_lens[b] > ctx) report_error(a.status, kErrBounds, b);  // a context longer than its block table
+  }
   if (a.table_out != nullptr && blockIdx.y == 0 && threadIdx.x == 0) a.table_out[blockIdx.x] = blockIdx.x;
   const int pages = (ctx + 15) / 16, filled = (max(pages, 1) + a.pad - 1) / a.pad * a.pad;
   if (p >= filled) return;
@@ -296,11 +301,16 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
 //     above 2^-33: long contexts have most of their mass in small weights. m moves
 //     only when a score exceeds it by 15 (2^15 fits f16), so most pages need no
 //     exchange between lanes and no rescaling.
+// Most pages that `tokens` neighbouring queries see through a window.
+__host__ __device__ inline int window_pages(int window, int tokens) {
+  return (int)(((long long)window + tokens - 1 + 14) / 16 + 1);
+}
+
 template <int D_, int NT_>
 struct Cfg {
   static constexpr int D = D_, NT = NT_, ROWS = 8 * NT_, STEPS = D_ / 16;
   static constexpr int PAGE = 16 * D_, STAGE = 2 * PAGE;
-  static constexpr int PP = NT_ == 1 ? 2 : 1;    // pages a warp works on at once
+  static constexpr int PP = NT_ <= 2 ? 2 : 1;    // pages a warp works on at once
   static constexpr int CTAS = 2;                 // resident per SM (registers)
     // Pages on their way per warp. Deeper rings are slower: 3 pages of 4 KB for each of 8 warps of an SM already fill
   // the memory system, and what is asked for beyond only delays block ids, scales and queries behind it (64 requests
@@ -314,7 +324,7 @@ struct Cfg {
 };
 
 struct SeqInfo {
-  int ctx, n, q0, lo, pages, rb;
+  int ctx, n, q0, pages, rb;  // pages: units of each of the rb blocks of query rows, at least the pages it sees
 };
 
 template <int ROWS>
@@ -329,11 +339,31 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedInt8Args& a, int b) {
     s.q0 = b;
     s.n = 1;
   }
-  s.lo = 0;
-  if (a.window > 0) s.lo = max(0, s.ctx - s.n - a.window + 1) / 16;
-  s.pages = (s.ctx + 15) / 16 - s.lo;
+  s.pages = (s.ctx + 15) / 16;
+  if (a.window > 0) s.pages = min(s.pages, window_pages(a.window, min(s.n, (ROWS - 1) / a.G + 2)));
   s.rb = (s.n * a.G + ROWS - 1) / ROWS;
   return s;
+}
+
+// Pages [lo, hi) that the rows of block rb see.
+struct PageRange {
+  int lo, hi;
+};
+
+template <int ROWS>
+__device__ __forceinline__ PageRange page_range(const PagedInt8Args& a, const SeqInfo& s, int rb) {
+  const int pos0 = s.ctx - s.n, first = pos0 + rb * ROWS / a.G;
+  const int last = pos0 + min(s.n * a.G - 1, rb * ROWS + ROWS - 1) / a.G;
+  PageRange r;
+  r.lo = a.window > 0 ? max(0, first - a.window + 1) / 16 : 0;
+  r.hi = max(r.lo, last < 0 ? 0 : last / 16 + 1);
+  return r;
+}
+
+// A context longer than its block table, or more queries than max_q_len: what does not fit is left out, and reported.
+__device__ __forceinline__ void check_seq(const PagedInt8Args& a, int b) {
+  const int n = a.cu_q != nullptr ? a.cu_q[b + 1] - a.cu_q[b] : 1;
+  if (a.ctx_lens[b] > (int64_t)a.max_blocks * 16 || n > a.max_q_len) report_error(a.status, kErrBounds, b);
 }
 
 constexpr int kWholePages = 16;
@@ -422,6 +452,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       if (b < a.B) {
         const SeqInfo s = seq_info<ROWS>(a, b);
         mine += a.Hkv * s.rb * s.pages;
+        if (blockIdx.x == 0) check_seq(a, b);
       }
     }
     int inc = mine;
@@ -463,8 +494,9 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
     u1 = min(u0 + chunk, U);
   }
 
-  // ---- the part of a segment at hand: units [u, ue) of [seg0, seg1), its first page, its rows ----
+  // ---- the part of a segment at hand: units [u, ue) of [seg0, seg1), of which cnt hold pages that its rows see ----
   int u = u0, ue, seg0, seg1, page, cnt;
+  int at = 0;  // pages of this warp before this part
   int b, h, row0, nrows, pos0, first_pos, last_pos, q0;
   const int32_t* tab;
   int seg = worker;  // (whole) the segment at hand
@@ -499,7 +531,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       }
     }
   };
-  int ui = u0;                                           // next unit to be asked for
+  int asked = 0;                                         // pages of this warp asked for so far
   uint32_t in_slot = 0, out_slot = 0, out_phase = 0;     // ring positions
   auto issue = [&](int y) {
     if (lane == 0) {
@@ -509,7 +541,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       tma_load_2d(dst + C::PAGE, &tmV, &full[in_slot], 0, y);
     }
     in_slot = in_slot + 1 == NST ? 0 : in_slot + 1;
-    ++ui;
+    ++asked;
   };
   auto next_slot = [&]() {
     if (++out_slot == NST) {
@@ -532,6 +564,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       h = hs / rb_max;
       rb = hs % rb_max;
       sq = seq_info<ROWS>(a, b);
+      if (lane == 0 && hs == 0) check_seq(a, b);
       seg0 = u;
       seg1 = ue = u + (rb < sq.rb ? sq.pages : 0);
     } else {
@@ -542,8 +575,9 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       seg1 = seg0 + sq.pages;
       ue = seg1 < u1 ? seg1 : u1;
     }
-    cnt = ue - u;
-    page = sq.lo + u - seg0;
+    const PageRange r = page_range<ROWS>(a, sq, rb);
+    page = r.lo + u - seg0;
+    cnt = max(0, min(ue - u, r.hi - page));
     tab = a.tables + (int64_t)b * a.max_blocks + page;
     row0 = rb * ROWS;
     nrows = min(ROWS, sq.n * a.G - row0);
@@ -555,20 +589,24 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
   auto peek = [&]() {  // at the part behind this one
     n_cnt = 0;
     if (a.whole ? seg + workers < segments : ue < u1) {
-      int nb = b, hs;
+      int nb = b, hs, rb, units;
       SeqInfo sq;
       if (a.whole) {
         nb = (seg + workers) / (a.Hkv * rb_max);
         hs = (seg + workers) % (a.Hkv * rb_max);
         sq = seq_info<ROWS>(a, nb);
         n_h = hs / rb_max;
-        n_cnt = hs % rb_max < sq.rb ? sq.pages : 0;
+        rb = hs % rb_max;
+        units = rb < sq.rb ? sq.pages : 0;
       } else {
         segment_of(ue, nb, sq, hs);
         n_h = hs / sq.rb;
-        n_cnt = min(sq.pages, u1 - ue);
+        rb = hs % sq.rb;
+        units = min(sq.pages, u1 - ue);
       }
-      n_id = lane < n_cnt ? a.tables[(int64_t)nb * a.max_blocks + sq.lo + lane] : 0;
+      const PageRange r = page_range<ROWS>(a, sq, rb);
+      n_cnt = max(0, min(units, r.hi - r.lo));
+      n_id = lane < n_cnt ? a.tables[(int64_t)nb * a.max_blocks + r.lo + lane] : 0;
     }
   };
   // Q: rows n = g of each tile in the order of the K fragments, scaled to below 2. The rows are asked for as soon as
@@ -638,7 +676,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
     // ids of the first 32 pages are here or on their way; some of the pages may have been asked for already
     resolve(0, y0, sk0, sv0);
 #pragma unroll 1
-    while (ui < ue && ui < u + NST) issue(__shfl_sync(0xffffffffu, y0, ui - u));
+    while (asked - at < min(cnt, NST)) issue(__shfl_sync(0xffffffffu, y0, asked - at));
     load_ids(32);
     place_q();
     peek();
@@ -675,7 +713,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
         if (p == 0 || j + p < cnt) {
           if (!mbar_wait(&full[out_slot], out_phase, a.status, kErrTimeoutFull)) {
             // copies in flight land before the CTA leaves (those behind the one given up on)
-            for (int k = u + j + p + 1; k < ui; ++k) {
+            for (int k = at + j + p + 1; k < asked; ++k) {
               next_slot();
               if (!mbar_wait(&full[out_slot], out_phase, a.status, kErrTimeoutDrain)) break;
             }
@@ -720,7 +758,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       __syncwarp();
 #pragma unroll
       for (int p = 0; p < PP; ++p) {
-        const int i = ui - u;  // page of this part, or of the next one
+        const int i = asked - at;  // page of this part, or of the next one
         if (i < min(j + PP, cnt) + NST) {  // (an odd last page frees one slot only)
           if (i < cnt) {
             issue(__shfl_sync(0xffffffffu, (i ^ j) < 32 ? y0 : y1, i));
@@ -882,6 +920,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       }
     }
     u = ue;
+    at += cnt;
     seg += workers;
     if (a.whole ? seg >= segments : u >= u1) break;
     locate();
@@ -1032,9 +1071,8 @@ static int ctas_per_sm(int nt) {
 static int tiles(int G, int max_q_len) { return std::min(4, (G * max_q_len + 7) / 8); }
 
 // pages of a segment that the host can rule out beyond, and whether warps take whole segments
-static int most_pages(int window, int max_q_len, int max_blocks) {
-  const int64_t keys = (int64_t)window + max_q_len - 1;
-  return window > 0 ? (int)std::min<int64_t>(max_blocks, (keys + 15) / 16 + 1) : max_blocks;
+static int most_pages(int nt, int G, int window, int max_q_len, int max_blocks) {
+  return window > 0 ? std::min(max_blocks, window_pages(window, std::min(max_q_len, (8 * nt - 1) / G + 2))) : max_blocks;
 }
 
 static int grid_ctas(int nt, int device, int B, int Hkv, int G, int max_q_len, int pages, bool whole) {
@@ -1063,7 +1101,7 @@ static void run(const PagedInt8Args& a, int grid, cudaStream_t st) {
 
 int64_t paged_int8_ws_floats(int device, int B, int Hkv, int G, int D, int max_q_len, int max_blocks, int window) {
   using namespace kv8;
-  const int nt = tiles(G, max_q_len), pages = most_pages(window, max_q_len, max_blocks);
+  const int nt = tiles(G, max_q_len), pages = most_pages(nt, G, window, max_q_len, max_blocks);
   if (pages <= kWholePages) return 0;
   return (int64_t)grid_ctas(nt, device, B, Hkv, G, max_q_len, pages, false) * 4 * 2 * 8 * nt * (D + 2) + B + 1;
 }
@@ -1073,7 +1111,7 @@ int paged_int8_launch(const PagedInt8Args& args, cudaStream_t st) {
   PagedInt8Args a = args;
   if (a.B == 0 || a.T == 0 || a.max_q_len == 0) return 0;
   const int nt = tiles(a.G, a.max_q_len);
-  const int pages = most_pages(a.window, a.max_q_len, a.max_blocks);
+  const int pages = most_pages(nt, a.G, a.window, a.max_q_len, a.max_blocks);
   a.whole = pages <= kWholePages ? 1 : 0;
   const int grid = grid_ctas(nt, a.device, a.B, a.Hkv, a.G, a.max_q_len, pages, a.whole != 0);
   if ((int64_t)a.B * a.Hkv * (((int64_t)a.G * a.max_q_len + 8 * nt - 1) / (8 * nt)) * std::max(pages, 1) > INT32_MAX / 2)

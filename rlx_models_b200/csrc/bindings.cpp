@@ -694,6 +694,7 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   Tensor k_out = at::empty({B * ob, k_cache.size(1), 16, k_cache.size(3)}, opt);
   Tensor v_out = at::empty({B * ob, k_cache.size(1), 16, k_cache.size(3)}, opt);
   Tensor table_out = at::empty({B, ob}, block_tables.options());
+  Tensor ctx_out = ob > 0 ? at::empty({B}, ctx_lens.options()) : ctx_lens;
   b200::KvInt8DequantArgs a{};
   a.k_cache = k_cache.data_ptr<int8_t>();
   a.v_cache = v_cache.data_ptr<int8_t>();
@@ -704,6 +705,7 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   a.k_out = static_cast<__nv_bfloat16*>(k_out.data_ptr());
   a.v_out = static_cast<__nv_bfloat16*>(v_out.data_ptr());
   a.table_out = table_out.data_ptr<int32_t>();
+  a.ctx_out = ob > 0 ? ctx_out.data_ptr<int32_t>() : nullptr;
   a.num_blocks = k_cache.size(0);
   a.B = (int)B;
   a.max_blocks = (int)mb;
@@ -714,7 +716,7 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   a.status = status.data_ptr<int>();
   b200::kv_int8_dequant_launch(a, cur_stream(k_cache));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {k_out, v_out, table_out};
+  return {k_out, v_out, table_out, ctx_out};
 }
 
 // Decode and short multi-token attention over int8 pages, into `out_opt` or a new tensor; and
@@ -744,8 +746,8 @@ std::tuple<Tensor, int64_t> paged_attention_int8(const Tensor& q, const Tensor& 
   const bool ragged = cu_q.has_value() && cu_q->defined();
   if (ragged) {
     TORCH_CHECK(cu_q->scalar_type() == at::kInt && cu_q->numel() == B + 1 && cu_q->is_contiguous() &&
-                    cu_q->device() == q.device() && max_q_len >= 0 && max_q_len * (Hq / Hkv) <= 65535,
-                "b200.paged_attention_int8: cu_q int32 [B + 1] and at most 65535 query rows per KV head");
+                    cu_q->device() == q.device() && max_q_len >= 0 && max_q_len * (Hq / Hkv) <= 8 * 65535,
+                "b200.paged_attention_int8: cu_q int32 [B + 1] and at most 524280 query rows per KV head");
   } else {
     TORCH_CHECK(T == B && max_q_len == 1, "b200.paged_attention_int8: one query per sequence without cu_q");
   }

@@ -56,7 +56,10 @@ def save_prompt(engine, path: str, tokens: list[int]) -> int:
     blocks = engine.sched.prefix_blocks(tokens)
     n = len(blocks)
     kv = engine.kv
-    tensors = {name: t.cpu() if n else torch.empty(0) for name, t in kv.gather_blocks(blocks).items()}
+    if n:
+        tensors = {name: t.cpu() for name, t in kv.gather_blocks(blocks).items()}
+    else:
+        tensors = {"k": torch.empty(0), "v": torch.empty(0)}
     tensors["tokens"] = torch.tensor(tokens[:n * BLOCK_SIZE], dtype=torch.int32)
     meta = {"format": FORMAT, "fingerprint": model_fingerprint(engine.model, kv), "blocks": str(n)}
     save_file(tensors, path, metadata=meta)

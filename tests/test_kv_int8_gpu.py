@@ -87,9 +87,9 @@ def check(out, want, mass, weight_eps):
 F16_EPS, BF16_EPS = 2.0 ** -11, 2.0 ** -8
 
 
-def weight_eps(hq, hkv, n):
+def weight_eps(hq, hkv, n, d=128):
     """Pages read directly: weights in f16. Through bf16 copies: ``prefill_attention`` rounds them to bf16."""
-    copies = n * hq > ops.INT8_DIRECT_ROWS * hkv and 128 * hkv % hq == 0
+    copies = n * hq > ops.INT8_DIRECT_ROWS * hkv and d == 128 and 8 * hkv % hq == 0
     return BF16_EPS if copies else F16_EPS
 
 DECODE = [1, 15, 16, 17, 100, 513, 2047]
@@ -131,24 +131,57 @@ def test_several_queries(cuda, hq, hkv, d, new, window):
                              scale=d ** -0.5, window=window, out=out)
     ops.check_errors(cuda)
     want, mass = oracle(q[:cu[-1]], cache, tables, lens, cu, d ** -0.5, window)
-    check(out[:cu[-1]], want, mass, weight_eps(hq, hkv, max(new)))
+    check(out[:cu[-1]], want, mass, weight_eps(hq, hkv, max(new), d))
     assert bool((out[cu[-1]:] == 7.0).all())
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (64, 8, 64), (6, 2, 64), (3, 1, 128)])
-def test_chunks(cuda, hq, hkv, d):
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (64, 8, 64), (6, 2, 64), (3, 1, 128), (16, 1, 128)])
+@pytest.mark.parametrize("window,sinks,cap", [(0, False, 0.0), (20, True, 0.0), (128, False, 0.0), (0, True, 15.0)])
+def test_chunks(cuda, hq, hkv, d, window, sinks, cap):
     lens, new = [300, 129, 77], [130, 129, 1]
     g = torch.Generator().manual_seed(5)
     tables, nb = make_tables(lens, g)
     cache = make_cache(cuda, nb, hkv, d, g)
     cu = [0, 130, 259, 260]
+    sk = torch.randn(hq, generator=g).to(cuda) if sinks else None
     q = (torch.randn(260, hq, d, generator=g) * 0.5).to(cuda, BF)
     out = ops.paged_attention_int8(q, *cache, tables.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda),
                                    cu_q=torch.tensor(cu, dtype=torch.int32, device=cuda), max_q_len=130,
-                                   scale=d ** -0.5)
+                                   scale=d ** -0.5, window=window, sinks=sk, softcap=cap)
     ops.check_errors(cuda)
-    want, mass = oracle(q, cache, tables, lens, cu, d ** -0.5)
-    check(out, want, mass, weight_eps(hq, hkv, 130))
+    want, mass = oracle(q, cache, tables, lens, cu, d ** -0.5, window, sk, cap)
+    check(out, want, mass, F16_EPS if cap else weight_eps(hq, hkv, 130, d))
+
+
+def test_chunks_in_groups(cuda, monkeypatch):
+    """Wide block tables: the bf16 copies are made for a few sequences at a time."""
+    lens, new = [300, 0, 129, 77], [130, 0, 129, 40]
+    g = torch.Generator().manual_seed(6)
+    tables, nb = make_tables(lens, g)
+    cache = make_cache(cuda, nb, 2, 128, g)
+    cu = [0, 130, 130, 259, 299]
+    q = (torch.randn(299, 8, 128, generator=g) * 0.5).to(cuda, BF)
+    args = (q, *cache, tables.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda))
+    kw = dict(cu_q=torch.tensor(cu, dtype=torch.int32, device=cuda), max_q_len=130, scale=0.1)
+    whole = ops.paged_attention_int8(*args, **kw)
+    for limit in (1, 400000):
+        monkeypatch.setattr(ops, "INT8_COPY_BYTES", limit)
+        assert torch.equal(whole, ops.paged_attention_int8(*args, **kw))
+    ops.check_errors(cuda)
+
+
+def test_what_does_not_fit_is_reported(cuda):
+    """Contexts longer than the block table and more queries than ``max_q_len``."""
+    g = torch.Generator().manual_seed(17)
+    tables, nb = make_tables([40, 40], g)
+    cache = make_cache(cuda, nb, 2, 128, g)
+    for n, most, ctx in ((1, 1, 49), (3, 2, 40), (40, 40, 400)):
+        q = torch.randn(2 * n, 8, 128, generator=g).to(cuda, BF)
+        ops.paged_attention_int8(q, *cache, tables.to(cuda), torch.tensor([40, ctx], dtype=torch.int32, device=cuda),
+                                 cu_q=torch.tensor([0, n, 2 * n], dtype=torch.int32, device=cuda), max_q_len=most,
+                                 scale=0.1)
+        with pytest.raises(ops.KernelError, match="bounds"):
+            ops.check_errors(cuda)
 
 
 @pytest.mark.parametrize("n", [1, 3, 40])
