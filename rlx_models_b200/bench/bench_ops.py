@@ -118,7 +118,7 @@ def wgrad(args, dev, timer, tf, hbm):
 
 
 def decode_attn_rows(args, cfg, dev, timer, hbm, rows, write=True):
-    """Decode attention over bf16 and float8 e4m3 pages (batch 64 at 1400 and
+    """Decode attention over bf16, float8 e4m3 and int8 pages (batch 64 at 1400 and
     2300 tokens of context; the pages spread over a cache larger than L2)."""
     Hq, Hkv, D = cfg.num_attention_heads // args.tp, cfg.num_key_value_heads // args.tp, cfg.head_dim
     for dt, esize, splits in ((torch.bfloat16, 2, 0), (torch.float8_e4m3fn, 1, 0), (torch.float8_e4m3fn, 1, 2),
@@ -141,6 +141,20 @@ def decode_attn_rows(args, cfg, dev, timer, hbm, rows, write=True):
                              us=round(t * 1e6, 1), tbs=round(byts / t / 1e12, 2),
                              frac_hbm=round(byts / t / 1e12 / hbm, 3)))
             print(json.dumps(rows[-1]), flush=True)
+    for (B, ctx) in ((64, 1400), (64, 2300)):
+        nbps = (ctx + 15) // 16
+        kc, vc = (torch.randint(-127, 128, (B * nbps, Hkv, 16, D), dtype=torch.int8, device=dev) for _ in range(2))
+        sc = torch.full((B * nbps, Hkv), 2.0 ** -6, device=dev)
+        tables = torch.randperm(B * nbps, device=dev).view(B, nbps).int()
+        ctxs = torch.full((B,), ctx, dtype=torch.int32, device=dev)
+        q = torch.randn(B, Hq, D, device=dev).bfloat16()
+        out = torch.empty_like(q)
+        t = timer(lambda: ops.paged_attention_int8(q, kc, vc, sc, sc, tables, ctxs, scale=1 / math.sqrt(D), out=out),
+                  args.reps)
+        byts = 2.0 * B * ctx * Hkv * D
+        rows.append(dict(op="decode_attn_int8", B=B, ctx=ctx, splits=0, us=round(t * 1e6, 1),
+                         tbs=round(byts / t / 1e12, 2), frac_hbm=round(byts / t / 1e12 / hbm, 3)))
+        print(json.dumps(rows[-1]), flush=True)
     if write and args.json:
         json.dump({"peaks": {"hbm_tbs": hbm}, "rows": rows}, open(args.json, "w"), indent=1)
 

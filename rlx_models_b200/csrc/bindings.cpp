@@ -637,9 +637,19 @@ static void check_int8_cache(const char* op, const Tensor& k, const Tensor& v, c
               "b200.", op, ": caches must be 16-byte aligned");
 }
 
-void kv_store_int8(const Tensor& k, const Tensor& v, const Tensor& slots, Tensor& k_cache, Tensor& v_cache,
+// Rows that the store reads as they are: contiguous, token and head strides of 16 bytes; others are copied.
+static Tensor aligned_rows(const Tensor& t) {
+  if (t.dim() != 3 || t.numel() == 0) return t;
+  const bool ok = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void kv_store_int8(const Tensor& k_in, const Tensor& v_in, const Tensor& slots, Tensor& k_cache, Tensor& v_cache,
                    Tensor& k_scale, Tensor& v_scale, Tensor& status) {
   check_int8_cache("kv_store_int8", k_cache, v_cache, k_scale, v_scale);
+  c10::cuda::CUDAGuard g(k_cache.device());
+  const Tensor k = aligned_rows(k_in), v = aligned_rows(v_in);
   const int64_t T = slots.numel(), Hkv = k_cache.size(1), D = k_cache.size(3);
   for (const Tensor* t : {&k, &v})
     TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 3 && t->size(0) == T && t->size(1) == Hkv &&
@@ -650,7 +660,6 @@ void kv_store_int8(const Tensor& k, const Tensor& v, const Tensor& slots, Tensor
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
                   slots.device() == k_cache.device(),
               "b200.kv_store_int8: slots int64 [T] on the caches' device");
-  c10::cuda::CUDAGuard g(k_cache.device());
   b200::KvInt8StoreArgs a{};
   a.k = static_cast<const __nv_bfloat16*>(k.data_ptr());
   a.v = static_cast<const __nv_bfloat16*>(v.data_ptr());
@@ -694,7 +703,8 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   Tensor k_out = at::empty({B * ob, k_cache.size(1), 16, k_cache.size(3)}, opt);
   Tensor v_out = at::empty({B * ob, k_cache.size(1), 16, k_cache.size(3)}, opt);
   Tensor table_out = at::empty({B, ob}, block_tables.options());
-  Tensor ctx_out = ob > 0 ? at::empty({B}, ctx_lens.options()) : ctx_lens;
+  const bool bound = pad > 1 && ob > 0;  // for attention over the copies: ctx_lens within the table
+  Tensor ctx_out = bound ? at::empty({B}, ctx_lens.options()) : ctx_lens;
   b200::KvInt8DequantArgs a{};
   a.k_cache = k_cache.data_ptr<int8_t>();
   a.v_cache = v_cache.data_ptr<int8_t>();
@@ -705,7 +715,7 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   a.k_out = static_cast<__nv_bfloat16*>(k_out.data_ptr());
   a.v_out = static_cast<__nv_bfloat16*>(v_out.data_ptr());
   a.table_out = table_out.data_ptr<int32_t>();
-  a.ctx_out = ob > 0 ? ctx_out.data_ptr<int32_t>() : nullptr;
+  a.ctx_out = bound ? ctx_out.data_ptr<int32_t>() : nullptr;
   a.num_blocks = k_cache.size(0);
   a.B = (int)B;
   a.max_blocks = (int)mb;

@@ -22,15 +22,17 @@
 // tiles of 512 tokens, the slice sums meet through distributed shared memory, and
 // the CTA whose slice holds the border walks its tiles.
 //
-// On a B200 a request with 4 drafts takes 18.5 us (the latency of the two launches
-// and a cluster's three meetings), 64 requests with up to 4 drafts 76 us: about 45
-// for the statistics, bound by instruction issue (29 a logit, 8 of them in 64 bits;
-// chunks of 4096 logits with more CTAs an SM are slower, 85 us in all).
+// On a B200 a request with 4 drafts takes 15.8 us (the latency of the two launches
+// and a cluster's three meetings; 1024 threads a CTA instead of 512: 16.5), 64
+// requests with up to 4 drafts 69 us: about 45 for the statistics, bound by
+// instruction issue (27 a logit, 8 of them in 64 bits; chunks of 4096 logits with
+// more CTAs an SM are slower), the rest for the draw from 64 rows of p and q.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include "../common/b200.cuh"
 #include "../common/launch.h"
@@ -323,41 +325,52 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, kBl
   const int64_t di = d0 + count;
   const bool rejected = count < n && di >= 0 && di < a.ND;  // (a draft outside its list: drawn from p)
   const float* q = rejected && a.probs != nullptr ? a.probs + di * a.ldp : nullptr;
-  const int gone = rejected && a.probs == nullptr ? a.drafts[di] : -1;  // a certain draft: q = 1 there
+  const int gone = rejected && a.probs == nullptr ? a.drafts[di] : INT32_MIN;  // a certain draft: q = 1 there
   const double inv = 1.0 / st.sum;
   const Exp64 ex(st.max, T, tab);
   bool plain = !rejected;
-  auto tile_weights = [&](int t, auto&& use) {  // use(i, w) of tokens t * kTile + i * 32 + lane
+  // use(i, w) of the 16 tokens at0 + i * step of a lane in tile t. A tile inside the row needs no bounds, and a row whose largest logit
+  // is an ordinary number no care for +inf (NaN and -inf fail `keep`).
+  auto tile_of = [&](int at0, auto step, auto careful, auto&& use) {
+    constexpr bool kCareful = decltype(careful)::value;
+    constexpr int kStep = decltype(step)::value;
+    const bool sub = !plain && q != nullptr;
     float xv[kLaneTile], qv[kLaneTile];
 #pragma unroll
-    for (int i = 0; i < kLaneTile; ++i) {
-      const int at = t * kTile + i * 32 + lane;
-      xv[i] = at < a.V ? x[at] : -INFINITY;
+    for (int i = 0; i < kLaneTile; ++i) xv[i] = !kCareful || at0 + i * kStep < a.V ? x[at0 + i * kStep] : -INFINITY;
+    if (sub) {
+#pragma unroll
+      for (int i = 0; i < kLaneTile; ++i) qv[i] = !kCareful || at0 + i * kStep < a.V ? q[at0 + i * kStep] : 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLaneTile; ++i) qv[i] = 0.f;
     }
+    const int skip = plain || gone < 0 ? -1 : gone - at0;
 #pragma unroll
     for (int i = 0; i < kLaneTile; ++i) {
-      const int at = t * kTile + i * 32 + lane;
-      qv[i] = !plain && q != nullptr && at < a.V ? q[at] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kLaneTile; ++i) {
-      const float xi = clean(xv[i]);
+      const float xi = kCareful ? clean(xv[i]) : xv[i];
       double scale, e;
       ex.parts(xi, scale, e);
-      const double v = fma(scale * e, inv, -(double)(qv[i] > 0.f ? qv[i] : 0.f));
-      const bool on = ex.keep(xi) && (plain || t * kTile + i * 32 + lane != gone);
-      use(i, on && v > 0.0 ? v : 0.0);
+      const double v = fma(scale * e, inv, -(double)fmaxf(qv[i], 0.f));  // (NaN counts as 0)
+      use(i, ex.keep(xi) && v > 0.0 && skip != i * kStep ? v : 0.0);
     }
+  };
+  using Spread = std::integral_constant<int, 32>;  // tokens of a lane 32 apart: coalesced loads
+  using InRow = std::integral_constant<int, 1>;    // one behind the other: a lane's running sum is in order
+  auto tile_weights = [&](int t, auto step, auto&& use) {
+    const int at0 = t * kTile + (decltype(step)::value == 32 ? lane : lane * kLaneTile);
+    if ((t + 1) * kTile <= a.V && st.max < FLT_MAX) tile_of(at0, step, std::false_type{}, use);
+    else tile_of(at0, step, std::true_type{}, use);
   };
   const int all_tiles = (a.V + kTile - 1) / kTile;
   const int per = (all_tiles + kCluster - 1) / kCluster;
   const int tile0 = min(rank * per, all_tiles), mine = min(tile0 + per, all_tiles) - tile0;
   const int seg = (mine + 31) / 32;  // tiles per lane, in order, where one warp adds them up
-  double total = 0.0;
+  double total = 0.0, slice = 0.0;
   for (int pass = 0; pass < 2; ++pass) {
     for (int t = warp; t < mine; t += kWarps) {
       double part[2] = {0.0, 0.0};
-      tile_weights(tile0 + t, [&](int i, double w) { part[i & 1] += w; });
+      tile_weights(tile0 + t, Spread{}, [&](int i, double w) { part[i & 1] += w; });
       const double sum = warp_sum(part[0] + part[1]);
       if (lane == 0) tiles[t] = sum;
     }
@@ -369,8 +382,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, kBl
       if (lane == 0) s_slice = s;
     }
     cluster.sync();
+    slice = lane < kCluster ? *cluster.map_shared_rank(&s_slice, lane) : 0.0;  // lane c: the sum of slice c
     total = 0.0;
-    for (int c = 0; c < kCluster; ++c) total += *cluster.map_shared_rank(&s_slice, c);
+    for (int c = 0; c < kCluster; ++c) total += __shfl_sync(0xffffffffu, slice, c);
     if (total > 0.0 || plain) break;
     plain = true;  // p == q up to rounding, yet refused: draw from p
     cluster.sync();
@@ -380,7 +394,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, kBl
   double before = 0.0, owner_before = 0.0;
   int owner = -1, fallback = 0;
   for (int c = 0; c < kCluster; ++c) {
-    const double s = *cluster.map_shared_rank(&s_slice, c);
+    const double s = __shfl_sync(0xffffffffu, slice, c);
     if (s > 0.0) fallback = c;
     if (owner < 0 && before + s > target) {
       owner = c;
@@ -423,21 +437,38 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, kBl
     }
     __syncwarp();
     const int t = tile0 + s_tile;
-    double sum = s_before;
-    int chosen = -1, tail = 0;
-    tile_weights(t, [&](int i, double w) {
-      double run = w;
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += v;
-      }
-      const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
-      if (some != 0) tail = t * kTile + i * 32 + 31 - __clz(some);
-      const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && sum + run > target);
-      if (over != 0 && s_end == 0 && chosen < 0) chosen = t * kTile + i * 32 + __ffs(over) - 1;
-      sum += __shfl_sync(0xffffffffu, run, 31);
+    double w[kLaneTile], own = 0.0;
+    int last_i = -1;
+    tile_weights(t, InRow{}, [&](int i, double v) {
+      w[i] = v;
+      own += v;
+      if (v > 0.0) last_i = i;
     });
-    if (lane == 0) out[count] = chosen >= 0 ? chosen : tail;
+    double run = own;
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += v;
+    }
+    // the lane that holds the border; behind every border (rounding): the last lane with weight, at its end
+    const unsigned some = __ballot_sync(0xffffffffu, last_i >= 0);
+    const unsigned over = s_end != 0 ? 0u : __ballot_sync(0xffffffffu, last_i >= 0 && s_before + run > target);
+    const int from = over != 0 ? __ffs(over) - 1 : (some != 0 ? 31 - __clz(some) : 0);
+    if (lane == from) {
+      double sum = s_before + run - own;
+      int pick = max(last_i, 0);
+      if (over != 0) {
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < kLaneTile; ++i) {
+          sum += w[i];
+          if (!found && w[i] > 0.0 && sum > target) {
+            pick = i;
+            found = true;
+          }
+        }
+      }
+      out[count] = t * kTile + lane * kLaneTile + pick;
+    }
   }
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }

@@ -323,7 +323,7 @@ def kv_store_int8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache
     """Quantise new rows into an int8 paged cache, in place.
 
     k / v bf16 [T, Hkv, D] (D 64 or 128; row views with 16-byte aligned strides
-    are read as they are), slots int64 [T] = block * 16 + offset, negative =
+    are read as they are, others copied), slots int64 [T] = block * 16 + offset, negative =
     skip; caches int8 [NB, Hkv, 16, D], scales fp32 [NB, Hkv]. Per (block, head):
     s = 2^e, the smallest e >= -100 with max|x| <= 127 s; code = rint(x / s). A
     block written at offset 0 starts over (offsets not written hold 0); any other
@@ -333,10 +333,6 @@ def kv_store_int8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache
 
     The tokens of one block must be adjacent in the batch; a slot that comes
     twice among them takes the later row."""
-    if k.stride(-1) != 1 or (k.stride(0) | k.stride(1)) % 8 or k.data_ptr() % 16:
-        k = k.clone(memory_format=torch.contiguous_format)
-    if v.stride(-1) != 1 or (v.stride(0) | v.stride(1)) % 8 or v.data_ptr() % 16:
-        v = v.clone(memory_format=torch.contiguous_format)
     _count(1)
     ext().kv_store_int8(k, v, slots, k_cache, v_cache, k_scale, v_scale, scratch(k_cache.device).status)
 
