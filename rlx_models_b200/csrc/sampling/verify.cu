@@ -75,12 +75,24 @@ __device__ __forceinline__ void fill_table(double* tab) {
 // e^((x - max) / T) for x <= max in 64 bits: y = (x - max) 512 / (T ln 2) = 512 n + j + r with |r| <= 1/2, so the value
 // is 2^n 2^(j / 512) e^z, z = r ln 2 / 512, |z| < 0.00068; Taylor to z^3 leaves z^4 / 24 < 9e-15 of it. Terms below
 // e^-700 are 0 (`keep`), and so are those of -inf and NaN.
+//
+// y is one fma of x, f and c = -f max rounded, so all values of one maximum are off by the same factor, which `fix`
+// takes out: the error of c, d = f max + c, is exact as an fma, and fix = e^(-d ln 2 / 512). A temperature below
+// |max| 2^-34 acts like that one: other fp32 values lie 2^-24 |max| and more below max, 2^10 temperatures, where terms
+// are 0 already. It bounds d by 2^-10, the terms of fix past the square by 4e-19.
 struct Exp64 {
   double f, c;  // y = f x + c
+  double fix;   // a kept term is fix times what `parts` gives
   float max, cut;
   const double* tab;
-  __device__ __forceinline__ Exp64(float mx, float T, const double* table)
-      : f(kTable * 1.44269504088896340736 / (double)T), c(-f * (double)mx), max(mx), cut(-700.f * T), tab(table) {}
+  __device__ __forceinline__ Exp64(float mx, float T, const double* table) : max(mx), tab(table) {
+    const float t = fmaxf(T, fabsf(mx) * 0x1p-34f);
+    f = kTable * 1.44269504088896340736 / (double)t;
+    c = -f * (double)mx;
+    const double z = fma(f, (double)mx, c) * (0.693147180559945309417 / kTable);
+    fix = 1.0 - z + 0.5 * z * z;
+    cut = -700.f * t;
+  }
   __device__ __forceinline__ bool keep(float x) const { return x - max > cut; }
   // scale * e^z without the range check
   __device__ __forceinline__ void parts(float x, double& scale, double& e) const {
@@ -103,7 +115,7 @@ struct Exp64 {
   __device__ __forceinline__ double operator()(float x) const {
     double scale, e;
     parts(x, scale, e);
-    return keep(x) ? scale * e : 0.0;
+    return keep(x) ? scale * e * fix : 0.0;
   }
 };
 
@@ -193,15 +205,15 @@ __global__ void __launch_bounds__(kStatThreads, 4) stats_kernel(VerifyArgs a) {
   if (sampled(T) && best != -INFINITY) {
     const Exp64 ex(best, T, tab);
     double part[2] = {0.0, 0.0};
-    const float low = best + ex.cut;
-    if (low < best) {  // terms below the cut enter as e^-700, which no sum of 1 and more sees (NaN loses)
+    const float low = __fadd_ru(best, ex.cut);  // (not below the cut: the exponent of 2^n stays in range)
+    if (low < best) {  // terms below it enter as e^-350 or less, which no sum of 1 and more sees (NaN loses)
 #pragma unroll
       for (int i = 0; i < kPerThread; ++i) ex.add(fmaxf(v[i], low), part[i & 1]);
+      sum = (part[0] + part[1]) * ex.fix;
     } else {  // so cold that only the maximum counts
 #pragma unroll
-      for (int i = 0; i < kPerThread; ++i) part[0] += v[i] == best ? 1.0 : 0.0;
+      for (int i = 0; i < kPerThread; ++i) sum += v[i] == best ? 1.0 : 0.0;
     }
-    sum = part[0] + part[1];
   }
   sum = warp_sum(sum);
   if ((tid & 31) == 0) s_sum[tid >> 5] = sum;
@@ -326,11 +338,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, kBl
   const bool rejected = count < n && di >= 0 && di < a.ND;  // (a draft outside its list: drawn from p)
   const float* q = rejected && a.probs != nullptr ? a.probs + di * a.ldp : nullptr;
   const int gone = rejected && a.probs == nullptr ? a.drafts[di] : INT32_MIN;  // a certain draft: q = 1 there
-  const double inv = 1.0 / st.sum;
   const Exp64 ex(st.max, T, tab);
+  const double inv = ex.fix / st.sum;
   bool plain = !rejected;
-  // use(i, w) of the 16 tokens at0 + i * step of a lane in tile t. A tile inside the row needs no bounds, and a row whose largest logit
-  // is an ordinary number no care for +inf (NaN and -inf fail `keep`).
+  // use(i, w) of the 16 tokens at0 + i * step of a lane. A tile inside the row needs no bounds, and a row whose largest
+  // logit is an ordinary number no care for +inf (NaN and -inf fail `keep`).
   auto tile_of = [&](int at0, auto step, auto careful, auto&& use) {
     constexpr bool kCareful = decltype(careful)::value;
     constexpr int kStep = decltype(step)::value;
@@ -436,7 +448,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, kBl
       }
     }
     __syncwarp();
-    const int t = tile0 + s_tile;
+    const int t = tile0 + max(s_tile, 0);
     double w[kLaneTile], own = 0.0;
     int last_i = -1;
     tile_weights(t, InRow{}, [&](int i, double v) {

@@ -57,6 +57,26 @@ def test_flat_and_peaked(cuda, spread):
     assert run(cuda, c) == want(c)
 
 
+@pytest.mark.parametrize("T", [1e-4, 1e-5, 3e-6, 1e-6, 1e-7, 3e-8, 1e-8, 3e-9, 1e-9, 1e-12, 1e-20, 1e-37, 1.4e-45])
+def test_cold(cuda, T):
+    """Temperatures at which neighbouring fp32 logits are many temperatures apart, next to ties of the largest: random
+    logits, logits a few of the last places apart around a power of two, and rows around 0."""
+    g = torch.Generator().manual_seed(11)
+    c = make(cuda, 9, 3, 9001, 4.0, g, greedy=0.0)
+    x, V = c["logits"], 9001
+    ulp = 2.0 ** -20  # of fp32 numbers from 8 up
+    for r in range(0, x.shape[0], 2):
+        x[r] = torch.randint(-9, 4, (V,), generator=g) * ulp + (16.0, -8.0, 0.0, 8.0)[r // 2 % 4]
+    for r in range(1, x.shape[0], 4):
+        x[r, torch.randint(0, V, (3,), generator=g)] = x[r].max()
+    c["temp"] = torch.full_like(c["temp"], T)
+    at = [r for b in range(9) for r in range(c["cu"][b], c["cu"][b + 1] - 1)]
+    c["drafts"] = x[at].argmax(1).int()
+    assert run(cuda, c) == want(c)
+    c["q"] = None
+    assert run(cuda, c) == want(c)
+
+
 def test_no_drafts_and_fewer_than_given(cuda):
     g = torch.Generator().manual_seed(4)
     c = make(cuda, 5, 0, 1000, 2.0, g)
