@@ -161,14 +161,14 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 6) store_kernel(KvInt8StoreA
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float f[4] = {bf16_lo(w[2 * j]), bf16_hi(w[2 * j]), bf16_lo(w[2 * j + 1]), bf16_hi(w[2 * j + 1])};
-          if (!finite) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) f[k] = f[k] != f[k] ? 0.f : fminf(fmaxf(f[k], -127.f * s), 127.f * s);
-          }
           // x / s is exact, so that adding 1.5 * 2^23 rounds it once, ties to even: the code is the low byte
           uint32_t q[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) q[k] = __float_as_uint(fmaf(f[k], inv, 12582912.f));
+          for (int k = 0; k < 4; ++k) {
+            float v = f[k] * inv;
+            if (!finite) v = v != v ? 0.f : fminf(fmaxf(v, -127.f), 127.f);
+            q[k] = __float_as_uint(v + 12582912.f);
+          }
           o[j] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
         }
       } else if (fresh) {
@@ -301,18 +301,13 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
 //     above 2^-33: long contexts have most of their mass in small weights. m moves
 //     only when a score exceeds it by 15 (2^15 fits f16), so most pages need no
 //     exchange between lanes and no rescaling.
-// Most pages that `tokens` neighbouring queries see through a window.
-__host__ __device__ inline int window_pages(int window, int tokens) {
-  return (int)(((long long)window + tokens - 1 + 14) / 16 + 1);
-}
-
 template <int D_, int NT_>
 struct Cfg {
   static constexpr int D = D_, NT = NT_, ROWS = 8 * NT_, STEPS = D_ / 16;
   static constexpr int PAGE = 16 * D_, STAGE = 2 * PAGE;
-  static constexpr int PP = NT_ <= 2 ? 2 : 1;    // pages a warp works on at once
-  static constexpr int CTAS = 2;                 // resident per SM (registers)
-    // Pages on their way per warp. Deeper rings are slower: 3 pages of 4 KB for each of 8 warps of an SM already fill
+  static constexpr int PP = NT_ <= 2 ? 2 : 1;  // pages a warp works on at once (more registers than that do not fit)
+  static constexpr int CTAS = 2;               // resident per SM (registers)
+  // Pages on their way per warp. Deeper rings are slower: 3 pages of 4 KB for each of 8 warps of an SM already fill
   // the memory system, and what is asked for beyond only delays block ids, scales and queries behind it (64 requests
   // of 512 to 2304 tokens, 12 warps an SM: 52.6 us with 4 pages, 47.6 with 3, 45.2 with 2; 8 warps with 3: 45.2).
   static constexpr int NST = 3 * (D_ == 64 ? 2 : 1);
@@ -322,6 +317,11 @@ struct Cfg {
   static constexpr int FIXED = RING + 4 * QBYTES + 4 * NST * 8 + 16;
   static constexpr int smem(int B) { return 1024 + FIXED + (B + 1) * 4; }
 };
+
+// Most pages that `tokens` neighbouring queries see through a window.
+__host__ __device__ inline int window_pages(int window, int tokens) {
+  return (int)(((long long)window + tokens - 1 + 14) / 16 + 1);
+}
 
 struct SeqInfo {
   int ctx, n, q0, pages, rb;  // pages: units of each of the rb blocks of query rows, at least the pages it sees

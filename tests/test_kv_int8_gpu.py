@@ -307,6 +307,23 @@ def test_store_is_exact(cuda, d, hkv):
     put(list(range(16)), x, y)
 
 
+def test_store_infinity_beside_the_largest_value(cuda):
+    """127 times the scale of bf16's largest value passes fp32: an infinity next to it is still +-127 steps."""
+    top = torch.finfo(BF).max
+    x = torch.zeros(2, 2, 64, dtype=BF)
+    x[0, 0, 0], x[0, 0, 1], x[0, 0, 2], x[0, 0, 3], x[1, 0, 4] = top, float("inf"), -float("inf"), -top, float("nan")
+    x[1, 1, 0], x[1, 1, 1] = -top, 1.0
+    slots = torch.tensor([16, 17])
+    cache = make_cache(cuda, 2, 2, 64, torch.Generator().manual_seed(0))
+    want = [t.cpu() for t in cache]
+    ops.kv_store_int8(x.to(cuda), x.to(cuda), slots.to(cuda), *cache)
+    for i in (0, 1):
+        ref.store_int8(x, slots, want[i], want[2 + i])
+    assert want[0][1, 0, 0, :4].tolist() == [64, 127, -127, -64]
+    for got, w in zip(cache, want):
+        assert torch.equal(got.cpu(), w)
+
+
 def test_store_reads_strided_rows(cuda):
     g = torch.Generator().manual_seed(8)
     fused = torch.randn(20, 12, 128, generator=g).to(cuda, BF)
