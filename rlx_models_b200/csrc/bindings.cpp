@@ -729,6 +729,39 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   return {k_out, v_out, table_out, ctx_out};
 }
 
+// The arguments of attention over int8 pages, whichever way it takes.
+void check_paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
+                                const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
+                                const optional<Tensor>& cu_q, int64_t max_q_len, const optional<Tensor>& sinks,
+                                int64_t window, const Tensor& out) {
+  check_int8_cache("paged_attention_int8", k_cache, v_cache, k_scale, v_scale);
+  check_int8_tables("paged_attention_int8", k_cache, block_tables, ctx_lens);
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.is_contiguous() &&
+                  q.size(2) == k_cache.size(3) && q.device() == k_cache.device(),
+              "b200.paged_attention_int8: q bf16 [T, Hq, D], contiguous, on the caches' device");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.sizes() == q.sizes() &&
+                  out.device() == q.device(),
+              "b200.paged_attention_int8: out like q");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) % 16 == 0,
+              "b200.paged_attention_int8: q and out must be 16-byte aligned");
+  const int64_t Hq = q.size(1), Hkv = k_cache.size(1), B = block_tables.size(0);
+  TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16,
+              "b200.paged_attention_int8: 1 to 16 query heads per KV head");
+  TORCH_CHECK(B <= 4096, "b200.paged_attention_int8: at most 4096 sequences");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX, "b200.paged_attention_int8: window >= 0");
+  if (cu_q.has_value() && cu_q->defined()) {
+    TORCH_CHECK(cu_q->scalar_type() == at::kInt && cu_q->numel() == B + 1 && cu_q->is_contiguous() &&
+                    cu_q->device() == q.device() && max_q_len >= 0 && max_q_len * (Hq / Hkv) <= 8 * 65535,
+                "b200.paged_attention_int8: cu_q int32 [B + 1] and at most 524280 query rows per KV head");
+  } else {
+    TORCH_CHECK(q.size(0) == B && max_q_len == 1, "b200.paged_attention_int8: one query per sequence without cu_q");
+  }
+  if (sinks.has_value() && sinks->defined())
+    TORCH_CHECK(sinks->scalar_type() == at::kFloat && sinks->numel() == Hq && sinks->is_contiguous() &&
+                    sinks->device() == q.device(),
+                "b200.paged_attention_int8: sinks f32 [Hq]");
+}
+
 // Decode and short multi-token attention over int8 pages, into `out_opt` or a new tensor; and
 // the number of launches.
 std::tuple<Tensor, int64_t> paged_attention_int8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
@@ -737,34 +770,13 @@ std::tuple<Tensor, int64_t> paged_attention_int8(const Tensor& q, const Tensor& 
                                                  const optional<Tensor>& cu_q, int64_t max_q_len, double scale,
                                                  const optional<Tensor>& sinks, int64_t window, double softcap,
                                                  const optional<Tensor>& out_opt, Tensor& status) {
-  check_int8_cache("paged_attention_int8", k_cache, v_cache, k_scale, v_scale);
-  check_int8_tables("paged_attention_int8", k_cache, block_tables, ctx_lens);
-  TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.is_contiguous() &&
-                  q.size(2) == k_cache.size(3) && q.device() == k_cache.device(),
-              "b200.paged_attention_int8: q bf16 [T, Hq, D], contiguous, on the caches' device");
+  check_cuda(q, "q");
   c10::cuda::CUDAGuard g(q.device());
   Tensor out = out_opt.has_value() && out_opt->defined() ? *out_opt : at::empty_like(q);
-  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.sizes() == q.sizes() &&
-                  out.device() == q.device(),
-              "b200.paged_attention_int8: out like q");
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) % 16 == 0,
-              "b200.paged_attention_int8: q and out must be 16-byte aligned");
+  check_paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q, max_q_len, sinks,
+                             window, out);
   const int64_t T = q.size(0), Hq = q.size(1), Hkv = k_cache.size(1), B = block_tables.size(0);
-  TORCH_CHECK(Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16, "b200.paged_attention_int8: 1 to 16 query heads per KV head");
-  TORCH_CHECK(B <= 4096, "b200.paged_attention_int8: at most 4096 sequences");
-  TORCH_CHECK(window >= 0 && window <= INT32_MAX, "b200.paged_attention_int8: window >= 0");
   const bool ragged = cu_q.has_value() && cu_q->defined();
-  if (ragged) {
-    TORCH_CHECK(cu_q->scalar_type() == at::kInt && cu_q->numel() == B + 1 && cu_q->is_contiguous() &&
-                    cu_q->device() == q.device() && max_q_len >= 0 && max_q_len * (Hq / Hkv) <= 8 * 65535,
-                "b200.paged_attention_int8: cu_q int32 [B + 1] and at most 524280 query rows per KV head");
-  } else {
-    TORCH_CHECK(T == B && max_q_len == 1, "b200.paged_attention_int8: one query per sequence without cu_q");
-  }
-  if (sinks.has_value() && sinks->defined())
-    TORCH_CHECK(sinks->scalar_type() == at::kFloat && sinks->numel() == Hq && sinks->is_contiguous() &&
-                    sinks->device() == q.device(),
-                "b200.paged_attention_int8: sinks f32 [Hq]");
   if (B == 0 || T == 0 || max_q_len == 0) return {out, 0};
   b200::PagedInt8Args a{};
   a.q = static_cast<const __nv_bfloat16*>(q.data_ptr());
@@ -1938,6 +1950,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_store_int8", &kv_store_int8);
   m.def("kv_dequant_pages_int8", &kv_dequant_pages_int8, py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"),
         py::arg("v_scale"), py::arg("block_tables"), py::arg("ctx_lens"), py::arg("status"), py::arg("pad") = 1);
+  m.def("check_paged_attention_int8", &check_paged_attention_int8);
   m.def("paged_attention_int8", &paged_attention_int8);
   m.def("kv_copy_blocks", &kv_copy_blocks);
   m.def("verify_drafts", &verify_drafts);

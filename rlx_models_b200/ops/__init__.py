@@ -331,8 +331,8 @@ def kv_store_int8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache
     rint(code * s_old / s'). NaN is stored as 0 and +-inf as +-127 s, neither
     counts in the maximum.
 
-    The tokens of one block must be adjacent in the batch; a slot that comes
-    twice among them takes the later row."""
+    The tokens of one block must be adjacent in the batch, without skipped rows
+    between them; a slot that comes twice among them takes the later row."""
     _count(1)
     ext().kv_store_int8(k, v, slots, k_cache, v_cache, k_scale, v_scale, scratch(k_cache.device).status)
 
@@ -372,13 +372,18 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     (D 128, groups of 1, 2, 4 or 8, no softcap). Measured on a B200, direct / by
     copies: 64 sequences of 1400 tokens, 64 rows 149 / 224 us, 128 rows 281 / 185
     us; 16 of 2400 tokens 74 / 106 and 124 / 76 us."""
-    if (cu_q is not None and max_q_len * q.shape[1] > INT8_DIRECT_ROWS * k_cache.shape[1] and q.shape[2] == 128
-            and 8 * k_cache.shape[1] % q.shape[1] == 0 and softcap <= 0 and block_tables.shape[1] > 0):
+    if window >= 16 * block_tables.shape[-1]:
+        window = 0  # no context passes it
+    if (cu_q is not None and max_q_len * q.shape[1] > INT8_DIRECT_ROWS * k_cache.shape[1] and q.shape[-1] == 128
+            and q.shape[1] in [g * k_cache.shape[1] for g in (1, 2, 4, 8)] and softcap <= 0
+            and block_tables.shape[-1] > 0):
         # copies of a sequence lie in a row and end on a multiple of 8 pages: one box of the kernel's loads. The table's
         # width decides how much memory they take: so many sequences at a time that it stays within INT8_COPY_BYTES
         status = scratch(q.device).status
         if out is None:
             out = torch.empty_like(q)
+        ext().check_paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q,
+                                         int(max_q_len), sinks, int(window), out)
         B, width = block_tables.shape
         group = max(1, INT8_COPY_BYTES // (4 * (width + 7) * k_cache[0].numel()))
         for i in range(0, B, group):

@@ -498,6 +498,47 @@ def test_same_result_every_time(cuda):
         assert torch.equal(first, ops.paged_attention_int8(q, *cache, tables.to(cuda), ctx, scale=0.1))
 
 
+def test_widest_window(cuda):
+    """The largest window is none, for queries in front of the first token too (which see nothing)."""
+    g = torch.Generator().manual_seed(21)
+    lens, n = [40, 3, 300], [5, 9, 80]
+    tables, nb = make_tables(lens, g)
+    cache = make_cache(cuda, nb, 2, 128, g)
+    cu = torch.tensor([0, 5, 14, 94], dtype=torch.int32, device=cuda)
+    q = torch.randn(94, 4, 128, generator=g).to(cuda, BF)
+    args = (tables.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda))
+    for longest in (9, 80):  # read directly, by copies
+        c, m = (cu[:3], 14) if longest == 9 else (cu, 94)
+        a = [t[:len(c) - 1] for t in args]
+        got = [ops.paged_attention_int8(q[:m], *cache, *a, cu_q=c, max_q_len=longest, scale=0.09, window=w)
+               for w in (0, 2 ** 31 - 1)]
+        assert torch.equal(*got) and not bool(got[1][5:11].any()) and bool(got[1][11:14].any(-1).all())
+    ops.check_errors(cuda)
+
+
+def test_chunk_refusals(cuda):
+    """The checks hold on the way through copies too; no head, no group."""
+    g = torch.Generator().manual_seed(22)
+    cache = make_cache(cuda, 8, 2, 128, g)
+    ok = dict(q=torch.zeros(100, 4, 128, dtype=BF, device=cuda), cu_q=torch.tensor([0, 100], dtype=torch.int32,
+              device=cuda), tables=torch.arange(8, dtype=torch.int32, device=cuda)[None], max_q_len=100,
+              ctx=torch.tensor([120], dtype=torch.int32, device=cuda))
+
+    def attend(q, tables, ctx, **kw):
+        return ops.paged_attention_int8(q, *cache, tables, ctx, scale=1.0, **kw)
+
+    attend(**ok)
+    bad = [dict(cu_q=ok["cu_q"].cpu()), dict(cu_q=ok["cu_q"].long()), dict(cu_q=torch.zeros(3, dtype=torch.int32,
+           device=cuda)), dict(ctx=ok["ctx"].cpu()), dict(sinks=torch.zeros(4)), dict(window=-1), dict(q=ok["q"].cpu()),
+           dict(out=torch.zeros(100, 512, dtype=BF, device=cuda)), dict(out=torch.zeros(100, 4, 128, dtype=BF)),
+           dict(q=ok["q"].half()), dict(q=ok["q"].transpose(0, 1)), dict(q=ok["q"][:, :0]), dict(q=ok["q"][:, :1]),
+           dict(max_q_len=1 << 20), dict(max_q_len=-1), dict(tables=ok["tables"].long())]
+    for kw in bad:
+        with pytest.raises(RuntimeError, match="b200"):
+            attend(**{**ok, **kw})
+    ops.check_errors(cuda)
+
+
 def test_refusals(cuda):
     g = torch.Generator().manual_seed(16)
     cache = make_cache(cuda, 4, 2, 64, g)
