@@ -144,9 +144,11 @@ class SpeculativeDecoder:
         """The draft model's token: its argmax, or a draw whose distribution is kept for the verification."""
         if self._gen is None:
             return int(logits.argmax())
-        q = torch.softmax(logits.float() / self._temperature, -1)
+        x = logits.double()  # (1 / temperature can pass fp32)
+        q = torch.nan_to_num(torch.softmax((x - x.amax()) / self._temperature, -1)).float()
         self._draft_probs.append(q)
-        return int(torch.multinomial(q, 1, generator=self._gen))
+        # exponential clocks: token i rings first with probability q_i
+        return int((q / torch.empty_like(q).exponential_(generator=self._gen)).argmax())
 
     def _verify(self, props: list[int], lv: torch.Tensor) -> tuple[list[int], int]:
         """Target logits [len(props) + 1, V] -> (accepted proposals and the token behind them, number accepted)."""
@@ -185,8 +187,8 @@ class SpeculativeDecoder:
         ``seed`` repeats."""
         t = self.target
         t.pos = 0
-        self._gen, self._temperature = None, float(temperature)
-        if temperature > 0:
+        self._gen, self._temperature = None, float(torch.tensor(temperature, dtype=torch.float32))
+        if self._temperature > 0:
             self._gen = torch.Generator(device=t.model.device).manual_seed(seed)
         if self.draft is not None:
             self.draft.pos = 0

@@ -51,3 +51,22 @@ def test_host_tensors_are_refused():
     with pytest.raises(RuntimeError):
         ops.paged_attention_int8(torch.zeros(1, 1, 64, dtype=torch.bfloat16), k, k, s, s,
                                  torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32), scale=1.0)
+
+
+def test_draft_draws_at_any_temperature():
+    """A draft model's draws: the largest logit when it is cold, nothing that raises when logits are not finite, and
+    the softmax's frequencies."""
+    from rlx_models_b200.runtime.speculative import SpeculativeDecoder
+    sd = SpeculativeDecoder.__new__(SpeculativeDecoder)
+    sd._gen, sd._draft_probs = torch.Generator().manual_seed(0), []
+    x = torch.tensor([1.0, 3.0, 2.0, -float("inf")])
+    for t in (1e-4, 1e-30, 1e-45, 1e-300):
+        sd._temperature = t
+        assert sd._pick(x) == 1 and sd._draft_probs[-1].tolist() == [0, 1, 0, 0]
+    sd._temperature = 1e30
+    assert sd._pick(x) != 3 and torch.allclose(sd._draft_probs[-1], torch.tensor([1, 1, 1, 0]) / 3)
+    assert 0 <= sd._pick(torch.full((4,), float("nan"))) < 4
+    sd._temperature, n = 1.5, 4000
+    p = torch.softmax(x.double() / 1.5, 0)
+    freq = torch.bincount(torch.tensor([sd._pick(x) for _ in range(n)]), minlength=4) / n
+    assert bool(((freq - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all())  # five standard deviations
