@@ -8,6 +8,7 @@
 // few bytes of a block's scales go with the first piece of its codes.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <stdexcept>
 
@@ -83,13 +84,12 @@ void kv_copy_blocks_launch(const KvCopyArgs& args, cudaStream_t st) {
   if (a.n == 0 || a.layers == 0 || a.parts == 0) return;
   int pieces = 0;
   for (int p = 0; p < a.parts; ++p) {
-    // the first part always has its own pieces, so there is a piece for the small ones to ride on
+    // the first part has its own pieces, for the small ones to ride on (an empty one: a launch of one piece)
     a.part[p].pieces = p > 0 && a.part[p].bytes < 1024 ? 0 : (int)((a.part[p].bytes + kPiece - 1) / kPiece);
     pieces += a.part[p].pieces;
   }
   if (pieces > 65535 || a.layers > 65535) throw std::runtime_error("b200.kv_copy_blocks: block or layer count too large");
-  if (pieces == 0) return;
-  launch_pdl(copy_kernel, dim3((unsigned)a.n, (unsigned)a.layers, (unsigned)pieces), dim3(kThreads), 0, st, a);
+  launch_pdl(copy_kernel, dim3((unsigned)a.n, (unsigned)a.layers, (unsigned)std::max(pieces, 1)), dim3(kThreads), 0, st, a);
 }
 
 }  // namespace b200

@@ -294,8 +294,8 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
 //     the constant -128 (page by page, so that nothing accumulates to cancel).
 //     2^24 and the block's K scale go into the factor of the scores, its V scale
 //     relative to the largest so far, s / s_ref, into the weights.
-//   * Q is scaled by a power of two per row to below 2, so that any bf16 row
-//     keeps its 8 bits in f16. P is rounded to f16 (2^-12 of each weight).
+//   * Q is scaled by a power of two per row to below 2, so that a bf16 row
+//     (below 2^116) keeps its 8 bits in f16. P is rounded to f16 (2^-12 of each weight).
 //   * weights are 2^(score - m) with m 8 below the running maximum, so that f16
 //     holds weights down to 2^-22 of the largest with all its bits and loses none
 //     above 2^-33: long contexts have most of their mass in small weights. m moves

@@ -452,6 +452,17 @@ def test_block_copies(cuda, int8, hkv):
     ops.kv_copy_blocks(src, src, [], [])
 
 
+def test_copy_small_blocks_beside_empty_ones(cuda):
+    src = [torch.zeros(2, 5, 0, device=cuda), torch.arange(30., device=cuda).view(2, 5, 3)]
+    dst = [torch.zeros_like(t) for t in src]
+    ops.kv_copy_blocks(src, dst, [1, 4], [0, 2])
+    want = torch.zeros(2, 5, 3, device=cuda)
+    want[:, [0, 2]] = src[1][:, [1, 4]]
+    assert torch.equal(dst[1], want)
+    ops.kv_copy_blocks(src[:1], dst[:1], [1], [0])
+    ops.check_errors(cuda)
+
+
 def test_streams_and_graphs(cuda):
     """A side stream, and two captured graphs of one shape whose replays alternate: every call has its own workspace."""
     g = torch.Generator().manual_seed(14)
