@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(Cfg<TILES>::THREADS, 1)
   uint64_t* p_full = s_full + 2;
   uint64_t* o_done = p_full + 2;
   uint64_t* s_free = o_done + 2;    // two tiles: the S buffer has been read by this one
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_free + 2);
+  uint64_t* join = s_free + 2;      // two tiles: the second may take its first turn
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(join + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_wait();
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(Cfg<TILES>::THREADS, 1)
       mbar_init(&o_done[i], 1);
       mbar_init(&s_free[i], 4);
     }
+    mbar_init(join, 1);
     fence_mbarrier_init();
   }
   if (warp == 1) {
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(Cfg<TILES>::THREADS, 1)
       auto wait_v = [&](int j) {
         return mbar_wait(&v_full[j % VS], (uint32_t)(j / VS) & 1, a.status, kErrTimeoutFull);
       };
-      auto mma_s = [&](int buf, int j) {
+      auto mma_s = [&](int buf, int j, bool alone) {
         const uint32_t qa = smem_u32(Qs) + t * kQ, kb = smem_u32(Ks) + j % KS * kKV;
         const uint32_t d = tmem + (TILES == 2 ? 0 : buf * kBN);
         tc_fence_after();
@@ -285,8 +287,9 @@ __global__ void __launch_bounds__(Cfg<TILES>::THREADS, 1)
         }
         umma_commit(&s_full[buf]);
         umma_commit(&k_empty[j % KS]);
+        if (TILES == 2 && alone) umma_commit(&k_empty[j % KS]);  // for the tile that takes no part
       };
-      auto mma_o = [&](int buf, int j, bool more) {
+      auto mma_o = [&](int buf, int j, bool more, bool alone) {
         const uint32_t pa = tmem + (TILES == 2 ? kPCol + t * (kBN / 2) : buf * kBN);
         const uint32_t vb = smem_u32(Vs) + j % VS * kKV;
         tc_fence_after();
@@ -296,21 +299,22 @@ __global__ void __launch_bounds__(Cfg<TILES>::THREADS, 1)
                       (more || kk > 0) ? 1u : 0u);
         umma_commit(&o_done[buf]);
         umma_commit(&v_empty[j % VS]);
+        if (TILES == 2 && alone) umma_commit(&v_empty[j % VS]);
       };
       bool ok = mbar_wait(q_full, 0, a.status, kErrTimeoutFull);
       if constexpr (TILES == 1) {
         ok = ok && wait_k(0);
-        if (ok) mma_s(0, 0);
+        if (ok) mma_s(0, 0, false);
         for (int j = 0; ok && j < n; ++j) {
           if (j + 1 < n) {
             // S buffer (j+1)&1 held P_{j-1}: wait until P_{j-1} V_{j-1} has completed
             if (j >= 1 && !mbar_wait(&o_done[(j - 1) & 1], ((j - 1) >> 1) & 1, a.status, kErrTimeoutAccEmpty)) break;
             if (!wait_k(j + 1)) break;
-            mma_s((j + 1) & 1, j + 1);
+            mma_s((j + 1) & 1, j + 1, false);
           }
           if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1, a.status, kErrTimeoutFull)) break;
           if (!wait_v(j)) break;
-          mma_o(j & 1, j, j > 0);
+          mma_o(j & 1, j, j > 0, false);
         }
       } else {
         // Tile t sees key tiles [lo[t], hi[t]); tile 0 begins and ends no later than tile 1. One thread issues the
@@ -326,31 +330,33 @@ __global__ void __launch_bounds__(Cfg<TILES>::THREADS, 1)
         auto read = [&](int i, int j) {  // tile i has read its S_j
           return mbar_wait(&s_free[i], (uint32_t)(j - lo[i]) & 1, a.status, kErrTimeoutAccEmpty);
         };
-        // Every turn of the other tile is waited for, also by a tile that takes no part yet: parities tell a turn from
-        // the next one, not from the one after.
+        // Parities tell a turn from the next one, not from the one after: whoever waits for a turn knows that the one
+        // before it is over. Tile 0 has waited for each turn of its own until tile 1 takes its first (`meet`), and then
+        // for each of tile 1, as tile 1 for each of tile 0. What tile 1 has not followed until then it is told by `join`.
+        const int meet = min(lo[1], hi[0] - 1);
         auto turn = [&](int j) {
-          const int other = 1 - t, before = t == 0 ? j - 1 : j;
-          if (sees(other, before)) return read(other, before);
-          return !sees(t, j) || !sees(t, j - 1) || read(t, j - 1);
+          if (t == 0) {
+            if (sees(1, j - 1) ? !read(1, j - 1) : sees(0, j - 1) && !read(0, j - 1)) return false;
+            if (j == meet) mbar_arrive(join);
+            return true;
+          }
+          if (j == lo[1]) return mbar_wait(join, 0, a.status, kErrTimeoutAccEmpty) && read(0, meet);
+          return sees(0, j) ? read(0, j) : read(1, j - 1);
         };
         auto next_s = [&](int j) {
+          if (!sees(t, j)) return true;
           if (!turn(j) || !wait_k(j)) return false;
-          if (sees(t, j)) mma_s(t, j);
-          else mbar_arrive(&k_empty[j % KS]);
+          mma_s(t, j, !sees(1 - t, j));
           return true;
         };
         auto next_o = [&](int j) {
-          if (!sees(t, j)) {
-            if (!wait_v(j)) return false;
-            mbar_arrive(&v_empty[j % VS]);
-            return true;
-          }
+          if (!sees(t, j)) return true;
           if (!mbar_wait(&p_full[t], (uint32_t)(j - lo[t]) & 1, a.status, kErrTimeoutFull) || !wait_v(j)) return false;
-          mma_o(t, j, j > lo[t]);
+          mma_o(t, j, j > lo[t], !sees(1 - t, j));
           return true;
         };
-        ok = ok && next_s(0);
-        for (int j = 0; ok && j < n; ++j) ok = (j + 1 == n || next_s(j + 1)) && next_o(j);
+        ok = ok && next_s(lo[t]);
+        for (int j = lo[t]; ok && j < hi[t]; ++j) ok = next_s(j + 1) && next_o(j);
       }
     }
   } else if (warp >= 4) {
@@ -560,7 +566,7 @@ void fmha_launch(const AttnArgs& a, cudaStream_t st) {
   };
   // Two query tiles a CTA where single ones would not find an SM each: one sequence over 8192 tokens with 148 tiles takes
   // 82 us in single ones, with 152 tiles 115 in pairs (two rounds of single ones would be 164).
-  if ((int64_t)a.B * q_tiles * a.Hkv > num_sms(a.device))
+  if (q_tiles > 1 && (int64_t)a.B * q_tiles * a.Hkv > num_sms(a.device))
     run(fmha_fwd_kernel<2>, 2, Cfg<2>::SMEM, Cfg<2>::THREADS);
   else
     run(fmha_fwd_kernel<1>, 1, Cfg<1>::SMEM, Cfg<1>::THREADS);

@@ -128,3 +128,21 @@ def test_two_tiles_in_a_graph_on_another_stream(cuda):
     side.synchronize()
     assert torch.equal(out, want)
     ops.check_errors(cuda)
+
+
+@pytest.mark.parametrize("window", [0, 48, 500])
+def test_second_tile_empty_or_apart(cuda, window):
+    """CTAs whose second tile has no tokens, or begins behind the first one's keys, many at once and again and again:
+    the thread that issues its products must neither miss a turn nor hold up the loads."""
+    g = torch.Generator().manual_seed(6)
+    n = [32] * 40 + [64] * 4 + [33, 1, 96, 128] * 4
+    lens = [l + 1400 for l in n]
+    q, k, v, tables, ctx, cu = make(cuda, lens, n, 32, 8, g)
+    cu_q = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    want = ops.prefill_attention(q, k, v, tables, ctx, cu_q, 128, scale=0.09, window=window)
+    check(want, q, k, v, tables, lens, cu, 0.09, window, None)
+    out = torch.empty_like(q)
+    for _ in range(60):
+        ops.prefill_attention(q, k, v, tables, ctx, cu_q, 128, scale=0.09, window=window, out=out)
+        assert torch.equal(out, want)
+    ops.check_errors(cuda)
