@@ -365,13 +365,17 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     ``max_q_len``), the last of its ``ctx_lens[b]`` tokens. ``sinks`` fp32 [Hq],
     ``window`` (0 = all) and ``softcap`` as in ``decode_attention``. A query that
     sees no key gives 0; rows of ``out`` behind cu_q[B] are left as they are.
+    A call repeats its bits; equal sequences of one batch may differ in the last
+    ones, for where a context is cut between warps depends on what lies before it.
 
     Up to ``INT8_DIRECT_ROWS`` query rows per KV head the pages are read as they
     are. Longer chunks are bound by their products and go through bf16 copies of
     the pages to the tcgen05 kernel of ``prefill_attention`` where it applies
-    (D 128, groups of 1, 2, 4 or 8, no softcap). Measured on a B200, direct / by
-    copies: 64 sequences of 1400 tokens, 64 rows 149 / 224 us, 128 rows 281 / 185
-    us; 16 of 2400 tokens 74 / 106 and 124 / 76 us."""
+    (D 128, groups of 1, 2, 4 or 8, no softcap). Measured on a B200 with 8 KV
+    heads, direct / by copies: 64 sequences of 1400 tokens, 64 rows 146 / 179 us,
+    80 rows 212 / 179 us; 16 of 2400 tokens 74 / 72 and 97 / 72 us. That kernel
+    does not split a context: few sequences are better off directly for longer (2
+    of 8192 tokens, 128 rows 66 / 96, 256 rows 103 / 98 us)."""
     if window >= 16 * block_tables.shape[-1]:
         window = 0  # no context passes it
     if (cu_q is not None and max_q_len * q.shape[1] > INT8_DIRECT_ROWS * k_cache.shape[1] and q.shape[-1] == 128
