@@ -32,7 +32,8 @@
 //                     every tile finds an SM of its own this is the shorter way.
 // Either way a row sees its tiles in the same order with the same arithmetic.
 // 2 x 1024 tokens over 8192, 32 / 8 heads: 397 us with one tile a CTA, 220 with
-// two (1170 TFLOP/s, in 256 CTAs on 148 SMs); 4 x 2048 from the start: 273 and 166.
+// two (1170 TFLOP/s, in 256 CTAs on 148 SMs, tensor pipes and exponential units 65%
+// busy); 4 x 2048 from the start: 273 and 166.
 // A key tile then takes about 3200 cycles for both: each softmax warp works through
 // 360 (scores to registers), 400 (maximum), 400 (the wait for the last product)
 // and 1500 cycles (exponentials, whose units it shares with the other tile).
