@@ -213,8 +213,10 @@ class Scheduler {
   // same full blocks. The partly filled block, which both would write, is
   // allocated anew: the caller copies its contents. Returns (new id, block to
   // copy, its copy), the blocks -1 when the last one is full. Tokens in flight
-  // must have been resolved.
-  std::tuple<int64_t, int32_t, int32_t> fork(int64_t id, int max_new_tokens) {
+  // must have been resolved. Without stop conditions of its own the branch has
+  // its parent's; they hold for the tokens it makes itself.
+  std::tuple<int64_t, int32_t, int32_t> fork(int64_t id, int max_new_tokens, std::optional<bool> ignore_eos,
+                                             const std::optional<std::vector<int32_t>>& stop_ids) {
     auto it = seqs_.find(id);
     if (it == seqs_.end() || it->second->status != RUNNING || it->second->pending > 0 || !is_decode(*it->second))
       throw std::invalid_argument("fork: the sequence is not decoding");
@@ -236,8 +238,8 @@ class Scheduler {
     s->prompt_len = p.prompt_len;
     s->num_computed = p.num_computed;
     s->max_new_tokens = max_new_tokens;
-    s->ignore_eos = p.ignore_eos;
-    s->stop_ids = p.stop_ids;
+    s->ignore_eos = ignore_eos.value_or(p.ignore_eos);
+    s->stop_ids = stop_ids.value_or(p.stop_ids);
     s->blocks.assign(p.blocks.begin(), p.blocks.begin() + full);
     for (int b : s->blocks) bm_.share(b);
     if (dst >= 0) s->blocks.push_back(dst);
@@ -622,7 +624,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("add_request", &Scheduler::add_request, py::arg("prompt"), py::arg("max_new_tokens"),
            py::arg("ignore_eos") = false, py::arg("stop_ids") = std::vector<int32_t>{})
       .def("abort", &Scheduler::abort)
-      .def("fork", &Scheduler::fork, py::arg("seq_id"), py::arg("max_new_tokens"))
+      .def("fork", &Scheduler::fork, py::arg("seq_id"), py::arg("max_new_tokens"), py::arg("ignore_eos") = py::none(),
+           py::arg("stop_ids") = py::none())
       .def("has_work", &Scheduler::has_work)
       .def("num_waiting", &Scheduler::num_waiting)
       .def("num_running", &Scheduler::num_running)

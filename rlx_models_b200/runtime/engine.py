@@ -293,7 +293,7 @@ class LLMEngine:
         """Branch a running request that has generated at least one token: a new
         request with the same prompt and the same output so far, which goes on by
         itself under ``params`` (default: the parent's; ``max_new_tokens`` counts
-        from the prompt). Both read the same full KV blocks; the partly filled
+        from the prompt, stop tokens hold from the branch on). Both read the same full KV blocks; the partly filled
         one is copied on the device. Returns the new request's id."""
         if self.stateful or self.cfg.kv_retrieval or hasattr(self.model, "share_tokens") \
                 or not hasattr(self.kv, "copy_blocks"):
@@ -307,7 +307,8 @@ class LLMEngine:
         params = params or st.params
         if st.prompt is None and (params.repetition_penalty != 1.0 or params.dry_multiplier > 0):
             raise ValueError("fork: the parent keeps no prompt for a repetition penalty or DRY")
-        child, src, dst = self.sched.fork(sid, int(params.max_new_tokens))
+        child, src, dst = self.sched.fork(sid, int(params.max_new_tokens), bool(params.ignore_eos),
+                                          list(params.stop_token_ids))
         if src >= 0:
             self.kv.copy_blocks([src], [dst])
         new = dataclasses.replace(st, seq_id=child, params=params, token_times=list(st.token_times),
