@@ -307,13 +307,15 @@ class LLMEngine:
         params = params or st.params
         if st.prompt is None and (params.repetition_penalty != 1.0 or params.dry_multiplier > 0):
             raise ValueError("fork: the parent keeps no prompt for a repetition penalty or DRY")
+        if params.logprobs and not st.params.logprobs:
+            raise ValueError("fork: the parent keeps no logprobs of the tokens so far")
         child, src, dst = self.sched.fork(sid, int(params.max_new_tokens), bool(params.ignore_eos),
                                           list(params.stop_token_ids))
         if src >= 0:
             self.kv.copy_blocks([src], [dst])
         new = dataclasses.replace(st, seq_id=child, params=params, token_times=list(st.token_times),
-                                  tokens=list(st.tokens), logprobs=list(st.logprobs), rng=None, mirostat_mu=None,
-                                  mirostat_lp2=None, out_counts=None)
+                                  tokens=list(st.tokens), logprobs=list(st.logprobs) if params.logprobs else [],
+                                  rng=None, mirostat_mu=None, mirostat_lp2=None, out_counts=None)
         if params.penalised or params.processed:
             new.out_counts = dict(collections.Counter(st.tokens))
         if new.mm is not None:

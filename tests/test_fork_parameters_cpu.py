@@ -39,6 +39,8 @@ class Host:
         for sid in sids:
             st = self.eng.requests[sid]
             st.tokens.append(token)
+            if st.params.logprobs:
+                st.logprobs.append(-0.5)
         for sid in s.update(sids, [token] * len(sids), EOS):
             self.out[sid], self.why[sid] = s.output_tokens(sid), s.finish_reason(sid)
         return sids
@@ -85,3 +87,22 @@ def test_scheduler_fork_keeps_the_parents_conditions_by_default():
     assert step(6) == [d]
     assert step(5) == [a, b]
     assert step(EOS) == [] and s.output_tokens(c) == [8, 6, 5, EOS]
+
+
+@pytest.mark.parametrize("parent,branch", [(True, True), (True, False), (False, False)])
+def test_logprobs_cover_every_token_or_none(parent, branch):
+    h = Host(P(max_new_tokens=8, ignore_eos=True, logprobs=parent))
+    h.step(10)
+    h.step(20)
+    b = h.eng.fork(h.a, P(max_new_tokens=8, ignore_eos=True, logprobs=branch))
+    h.step(30)
+    for sid, on in ((h.a, parent), (b, branch)):
+        assert len(h.eng.requests[sid].logprobs) == (3 if on else 0)
+
+
+def test_logprobs_that_the_parent_has_not_kept_are_refused():
+    h = Host(P(max_new_tokens=8, ignore_eos=True))
+    h.step(10)
+    with pytest.raises(ValueError, match="logprobs"):
+        h.eng.fork(h.a, P(max_new_tokens=8, logprobs=True))
+    assert h.eng.sched.num_running() == 1
