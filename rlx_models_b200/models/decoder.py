@@ -261,8 +261,8 @@ class DecoderLM:
                          inv_freq=L.inv_freq, rope_scale=L.rope_mult, rot_dim=self.cfg.rotary_dim,
                          q_norm=None if full else L.q_norm, k_norm=None if full else L.k_norm,
                          eps=self.cfg.rms_norm_eps, k_out=k, v_out=v, bias=bias)
+        kv.store_int8(i, k, v, fb.slots)
         cache = kv.int8_layer(i)
-        ops.kv_store_int8(k, v, fb.slots, *cache)
         o = torch.empty_like(q)
         kw = dict(scale=self.scale, sinks=L.sinks, window=L.window, softcap=self.cfg.attn_softcap)
         if nd > 0:

@@ -51,6 +51,15 @@ class PagedKVCache:
         """(k, v, k_scale, v_scale) of one layer of an int8 cache."""
         return self.k[i], self.v[i], self.k_scale[i], self.v_scale[i]
 
+    rows: list | None = None  # (k, v) of every ``store_int8`` while a list is here, to store them again
+
+    def store_int8(self, i: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """``ops.kv_store_int8`` into layer ``i``; ``rows`` keeps what was stored."""
+        from .. import ops
+        ops.kv_store_int8(k, v, slots, *self.int8_layer(i))
+        if self.rows is not None:
+            self.rows.append((k, v))
+
     def tensors(self) -> dict[str, torch.Tensor]:
         """Everything a block consists of, by name, each [L, num_blocks, ...]."""
         named = {"k": self.k, "v": self.v, "k_scale": self.k_scale, "v_scale": self.v_scale}

@@ -22,7 +22,14 @@ numbers); looked-up tokens and a learned head's count as certain drafts (q = 1).
 
 KV caches are positional (slot = position under an identity block table), so
 rolling back after a rejection is just moving the position: stale entries past
-it are overwritten by the next writes.
+it are overwritten by the next writes. In int8 pages a refused row has also
+raised its block's scale, which rounds the accepted rows again: there the partly
+filled block is kept aside before the drafts are stored, and put back after the
+pass with the accepted rows stored behind it one by one (``_Seq.roll_back``), so that
+the cache holds what decoding token by token would have left. Within one pass
+a block's scale takes all drafts in, so on int8 pages the logits of a token whose
+block ends in larger drafts carry a coarser rounding of its earlier rows than plain
+decoding would.
 
   * a learned draft head (runtime/draft_head.py): the target's own final
     features plus the newest token through one small layer, recurring on its
@@ -61,7 +68,8 @@ class _Seq:
     def __init__(self, model, max_len: int):
         self.model = model
         self.nb = (max_len + 15) // 16 + 1
-        self.kv = model.make_kv_cache(self.nb)
+        self.int8 = getattr(model, "kv_dtype", None) == torch.int8
+        self.kv = model.make_kv_cache(self.nb + int(self.int8))  # (int8: the last block is for ``mark``)
         dev = model.device
         self.table = torch.arange(self.nb, dtype=torch.int32, device=dev).view(1, -1)
         self.pos = 0  # positions [0, pos) hold valid K/V
@@ -90,6 +98,39 @@ class _Seq:
             out = self.model.forward(fb, self.kv)
         self.pos = ctx
         return out
+
+    def reset(self) -> None:
+        self.pos = 0
+        if self.int8:
+            self.kv.rows = None
+
+    def mark(self) -> None:
+        """Rows from here on may be rolled back."""
+        self.start = self.pos
+        if self.int8:
+            if self.start % 16:
+                self.kv.copy_blocks([self.start // 16], [self.nb])
+            self.kv.rows = []
+
+    def roll_back(self, end: int) -> None:
+        """Keep the rows since ``mark`` up to position ``end``, forget those behind it. int8 pages then hold
+        what storing the kept rows one by one leaves."""
+        if self.int8 and self.kv.rows and (end < self.pos or any(k.shape[0] > 1 for k, _ in self.kv.rows)):
+            from .. import ops
+            kv, n, layers = self.kv, min(end, self.pos) - self.start, self.kv.num_layers
+            if self.start % 16:
+                kv.copy_blocks([self.nb], [self.start // 16])
+            if n > 0:
+                # [layers, rows, ...]; all layers of a row in one launch, as blocks of one long cache
+                k, v = (torch.stack([torch.cat([r[i] for r in kv.rows[l::layers]])[:n] for l in range(layers)])
+                        for i in (0, 1))
+                cache = [t.flatten(0, 1) for t in kv.tensors().values()]
+                slots = torch.arange(layers, device=k.device) * (kv.num_blocks * 16) + self.start
+                for j in range(n):
+                    ops.kv_store_int8(k[:, j], v[:, j], slots + j, *cache)
+        if self.int8:
+            self.kv.rows = None
+        self.pos = min(self.pos, end)
 
 
 _STATE_ATTRS = ("conv", "rec", "ssm")  # per-slot recurrent state tensors [layers, slots, ...] of hybrid caches
@@ -133,6 +174,7 @@ class SpeculativeDecoder:
         # catch up: feed every accepted token the draft has not seen (the last one included)
         pending = seq[d.pos:]
         lg = d.run(pending, d.pos)
+        d.mark()
         self._draft_probs = []
         props = [self._pick(lg[-1])]
         for _ in range(k - 1):
@@ -186,12 +228,12 @@ class SpeculativeDecoder:
         """Greedy, or with ``temperature`` > 0 a draw from the target's softmax(logits / temperature) that
         ``seed`` repeats."""
         t = self.target
-        t.pos = 0
+        t.reset()
         self._gen, self._temperature = None, float(torch.tensor(temperature, dtype=torch.float32))
         if self._temperature > 0:
             self._gen = torch.Generator(device=t.model.device).manual_seed(seed)
         if self.draft is not None:
-            self.draft.pos = 0
+            self.draft.reset()
         keep = self.head is not None
         lg = t.run(list(prompt), 0, keep)
         seq = list(prompt) + self._verify([], lg[-1:])[0]
@@ -207,6 +249,7 @@ class SpeculativeDecoder:
             # verify: the last accepted token (not yet in the target cache) + proposals
             start = len(seq) - 1
             snap = _snapshot(t.kv) if self.stateful and props else None
+            t.mark()
             lv = t.run([seq[-1]] + props, start, keep)
             new, n_acc = self._verify(props, lv)
             if snap is not None and n_acc < len(props):
@@ -220,7 +263,7 @@ class SpeculativeDecoder:
             new = new[:max_new_tokens - len(out)]
             seq += new
             out += new
-            t.pos = len(seq) - 1  # the newest token is not in the cache yet
+            t.roll_back(len(seq) - 1)  # the newest token is not in the cache yet
             if self.draft is not None:
-                self.draft.pos = min(self.draft.pos, len(seq) - 1)
+                self.draft.roll_back(len(seq) - 1)
         return out
