@@ -882,7 +882,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
     // ---- the rows of this part: out, or to the workspace ----
     const bool whole = seg0 >= u0 && seg1 <= u1;
     float* part = a.ws + ((int64_t)worker * 2 + (seg0 < u0 ? 0 : 1)) * ROWS * (D + 2);
-    const float unit = sref * 16777216.f;
+    // O 2^24 / sum is a mean of codes; the unit, up to 2^122, comes behind it, so that nothing passes fp32 on the way
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -895,7 +895,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
         if (r < nrows) {
           if (whole) {
             const int rr = row0 + r, head = h * a.G + rr % a.G;
-            float f = unit;
+            float f = 16777216.f;
             if (a.sinks != nullptr) {
               const float sk2 = a.sinks[head] * kLog2e, top = fmaxf(m[nt][c], sk2), fm = ex2(m[nt][c] - top);
               sum = sum * fm + ex2(sk2 - top);
@@ -905,12 +905,15 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
             __nv_bfloat16* dst = a.out + ((int64_t)(q0 + rr / a.G) * a.Hq + head) * D + 2 * g;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
-              *reinterpret_cast<uint32_t*>(dst + 16 * s) = pack_bf16x2(o[nt][s][c] * f, o[nt][s][2 + c] * f);
+              *reinterpret_cast<uint32_t*>(dst + 16 * s) =
+                  pack_bf16x2(o[nt][s][c] * f * sref, o[nt][s][2 + c] * f * sref);
           } else {
+            const float f = sum == 0.f ? 0.f : 16777216.f / sum;
             float* dst = part + r * D + 2 * g;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
-              *reinterpret_cast<float2*>(dst + 16 * s) = make_float2(o[nt][s][c] * unit, o[nt][s][2 + c] * unit);
+              *reinterpret_cast<float2*>(dst + 16 * s) =
+                  make_float2(o[nt][s][c] * f * sref, o[nt][s][2 + c] * f * sref);
             if (g == 0) {
               part[ROWS * D + r] = m[nt][c];
               part[ROWS * D + ROWS + r] = sum;
@@ -930,10 +933,13 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
 }
 
 // Joins the parts of the segments that several warps share and writes zeros for
-// rows without keys. D / 4 lanes hold a row; with few rows several such groups
-// share a row's parts (a context that is cut over many CTAs has few rows next to
-// it), with many a CTA takes as many rows as it has groups.
+// rows without keys. A part is the mean of its values, its maximum and its sum of
+// weights: means are averaged, so that no value passes the largest one. D / 4 lanes
+// hold a row; with few rows several such groups share a row's parts (a context that
+// is cut over many CTAs has few rows next to it), with many a CTA takes as many rows
+// as it has groups.
 constexpr int kMergeThreads = 256;
+constexpr float kNothing = 1e-36f;  // sums of weights next to a sink that outweighs them by 2^100
 
 template <int D, int NT>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(PagedInt8Args a, int grid) {
@@ -984,25 +990,26 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(PagedInt8Args a, i
       float mx = top;
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) mx = fmaxf(mx, pm[k]);
-      const float f = ex2(top - mx);
+      const float f = ex2(top - mx), old = sum * f;
       sink *= f;
-      sum *= f;
-      acc.x *= f;
-      acc.y *= f;
-      acc.z *= f;
-      acc.w *= f;
       top = mx;
+      sum = old;
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
-        const float w = i + k * ways <= i1 ? ex2(pm[k] - top) : 0.f;
-        sum += w * pl[k];
+        pl[k] *= ex2(pm[k] - top);
+        sum += pl[k];
+      }
+      const float inv = sum < kNothing ? 0.f : 1.f / sum, keep = old * inv;
+      acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const float w = pl[k] * inv;
         acc.x += w * v[k].x;
         acc.y += w * v[k].y;
         acc.z += w * v[k].z;
         acc.w += w * v[k].w;
       }
     }
-    if (way == 0) sum += sink;
     m_own = top;
   }
   if (ways > 1) {
@@ -1012,17 +1019,16 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(PagedInt8Args a, i
     if (join && way == 0) {  // (rows * ways <= GROUPS: the groups of a row lie inside the arrays)
       float top = m_own;
       for (int w = 1; w < ways; ++w) top = fmaxf(top, s_ml[grp + w].x);
-      const float f0 = ex2(m_own - top);
-      sum *= f0;
-      acc.x *= f0;
-      acc.y *= f0;
-      acc.z *= f0;
-      acc.w *= f0;
+      const float f0 = ex2(m_own - top), own = sum * f0;
+      sink *= f0;
+      sum = own;
+      for (int w = 1; w < ways; ++w) sum += ex2(s_ml[grp + w].x - top) * s_ml[grp + w].y;
+      const float inv = sum < kNothing ? 0.f : 1.f / sum, keep = own * inv;
+      acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
       for (int w = 1; w < ways; ++w) {
         const float4 v = s_acc[tid + w * LANES];
         const float2 ml = s_ml[grp + w];
-        const float f = ex2(ml.x - top);
-        sum += f * ml.y;
+        const float f = ex2(ml.x - top) * ml.y * inv;
         acc.x += f * v.x;
         acc.y += f * v.y;
         acc.z += f * v.z;
@@ -1031,8 +1037,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(PagedInt8Args a, i
     }
   }
   if (join && way == 0) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *out = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    const float f = sum < kNothing ? 0.f : sum / (sum + sink);  // (the sink has no value)
+    *out = make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
   }
 }
 
