@@ -293,14 +293,18 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
 //     exactly: S starts at -128 sum(q), and O gets one more product per tile with
 //     the constant -128 (page by page, so that nothing accumulates to cancel).
 //     2^24 and the block's K scale go into the factor of the scores, its V scale
-//     relative to the largest so far, s / s_ref, into the weights.
+//     relative to a unit of the segment (the largest of its first 32 pages) into the
+//     weights.
 //   * Q is scaled by a power of two per row to below 2, so that a bf16 row
 //     (below 2^116) keeps its 8 bits in f16. P is rounded to f16 (2^-12 of each weight).
-//   * weights are 2^(score - m) with m 8 below the running maximum, so that f16
-//     holds weights down to 2^-22 of the largest with all its bits and loses none
-//     above 2^-33: long contexts have most of their mass in small weights. m moves
-//     only when a score exceeds it by 15 (2^15 fits f16), so most pages need no
-//     exchange between lanes and no rescaling.
+//   * weights are 2^(score - m) times the V scale, with m 8 below the running maximum
+//     of both, score + log2 of the scale, so that f16 holds products down to 2^-22 of
+//     the largest with all its bits and loses none above 2^-33: long contexts have most
+//     of their mass in small weights, and a page whose scale is far above or below the
+//     others' counts by what it adds to the result. Sums of weights are fp32 and may
+//     lie as far from 1 as the scales lie apart: up to 2^80 nothing is lost. m moves
+//     only when it is exceeded by 15 (2^15 fits f16), so most pages need no exchange
+//     between lanes and no rescaling.
 template <int D_, int NT_>
 struct Cfg {
   static constexpr int D = D_, NT = NT_, ROWS = 8 * NT_, STEPS = D_ / 16;
@@ -377,6 +381,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
@@ -404,6 +414,8 @@ constexpr uint32_t kMinus128 = 0x80808080u;  // f16x2 of -128 * 2^-24
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kShift = 8.f;  // m: the running maximum minus this (log2), see above
 constexpr float kLimit = 15.f;  // a score above m + kLimit moves m
+constexpr int kUnitExp = 60;    // the segment's unit lies within 2^-60 and 2^60, where sums of weights have room
+constexpr float kFarScale = 0x1p100f, kNearLog = -80.f;  // scales further from the unit than these count as these
 constexpr float kNone = -1e30f; // m before the first visible key: finite, so that a masked score (-inf) has weight 0
 
 // Byte offset of 16-byte chunk c of row r in a page written by TMA with the
@@ -689,7 +701,9 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) o[nt][s][0] = o[nt][s][1] = o[nt][s][2] = o[nt][s][3] = 0.f;
     }
-    float sref = 0.f, iref = 0.f;
+    const int sv_exp = __reduce_max_sync(0xffffffffu, __float_as_int(sv0) >> 23);
+    const int unit_exp = min(max(sv_exp, 127 - kUnitExp), 127 + kUnitExp);
+    const float unit = __int_as_float(unit_exp << 23), per_unit = __int_as_float((254 - unit_exp) << 23);
     int key0 = page * 16;
 #pragma unroll 1
     for (int j = 0; j < cnt; j += PP, key0 += 16 * PP) {
@@ -802,23 +816,29 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
               if (key > pos || (a.window > 0 && key <= pos - a.window) || j + p >= cnt) sc[p][nt][i] = -INFINITY;
             }
       }
+      // V scales in units, and the largest score of each row with their log2
+      float cv[PP], lv[PP];
+#pragma unroll
+      for (int p = 0; p < PP; ++p) {
+        cv[p] = fminf(sv[p] * per_unit, kFarScale);
+        lv[p] = fmaxf(lg2(cv[p]), kNearLog);
+      }
+      auto top = [&](int nt, int c) {
+        float mx = fmaxf(sc[0][nt][c], sc[0][nt][2 + c]) + lv[0];
+        if constexpr (PP == 2) mx = fmaxf(mx, fmaxf(sc[PP - 1][nt][c], sc[PP - 1][nt][2 + c]) + lv[PP - 1]);
+        return mx;
+      };
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(sc[0][nt][c], sc[0][nt][2 + c]);
-          if constexpr (PP == 2) mx = fmaxf(mx, fmaxf(sc[PP - 1][nt][c], sc[PP - 1][nt][2 + c]));
-          grow |= mx > m[nt][c] + kLimit;
-        }
+        for (int c = 0; c < 2; ++c) grow |= top(nt, c) > m[nt][c] + kLimit;
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(sc[0][nt][c], sc[0][nt][2 + c]);
-            if constexpr (PP == 2) mx = fmaxf(mx, fmaxf(sc[PP - 1][nt][c], sc[PP - 1][nt][2 + c]));
-            mx = fmaxf(m[nt][c], mx - kShift);
+            float mx = fmaxf(m[nt][c], top(nt, c) - kShift);
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -833,23 +853,11 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
           }
         }
       }
-      const float sv_max = PP == 2 ? fmaxf(sv[0], sv[PP - 1]) : sv[0];
-      if (sv_max > sref) {  // a larger V scale: the sums are kept in units of the largest
-        const float f = sref / sv_max;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[nt][s][i] *= f;
-        sref = sv_max;
-        iref = 1.f / sv_max;
-      }
       // weights, transposed to the operand order
       uint32_t pf[PP][NT][2];
 #pragma unroll
       for (int p = 0; p < PP; ++p) {
-        const float c = sv[p] * iref;
+        const float c = cv[p];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float p0 = ex2(sc[p][nt][0] - m[nt][0]), p1 = ex2(sc[p][nt][1] - m[nt][1]);
@@ -906,14 +914,14 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
               *reinterpret_cast<uint32_t*>(dst + 16 * s) =
-                  pack_bf16x2(o[nt][s][c] * f * sref, o[nt][s][2 + c] * f * sref);
+                  pack_bf16x2(o[nt][s][c] * f * unit, o[nt][s][2 + c] * f * unit);
           } else {
             const float f = sum == 0.f ? 0.f : 16777216.f / sum;
             float* dst = part + r * D + 2 * g;
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
               *reinterpret_cast<float2*>(dst + 16 * s) =
-                  make_float2(o[nt][s][c] * f * sref, o[nt][s][2 + c] * f * sref);
+                  make_float2(o[nt][s][c] * f * unit, o[nt][s][2 + c] * f * unit);
             if (g == 0) {
               part[ROWS * D + r] = m[nt][c];
               part[ROWS * D + ROWS + r] = sum;

@@ -30,3 +30,83 @@ def test_values_near_the_largest(cuda, d, n, sinks):
     assert bool(out.isfinite().all())
     want, mass = oracle(q, cache, tables, lens, cu, d ** -0.5, 0, sk)
     check(out, want, mass, F16_EPS)
+
+
+def far_oracle(q, cache, tables, lens, cu, scale, sinks=None):
+    """64-bit attention; sum_j p_j |v_j|; sum_j p_j s_j with s_j the V scale of the key's page."""
+    k, v, ks, vs = (t.cpu().double() for t in cache)
+    q, tables = q.cpu().double(), tables.long()
+    out, mass, unit = (torch.zeros_like(q) for _ in range(3))
+    G = q.shape[1] // k.shape[1]
+    for b, L in enumerate(lens):
+        n, at = cu[b + 1] - cu[b], tables[b, :(L + 15) // 16]
+        for h in range(q.shape[1]):
+            kk = (k[at, h // G] * ks[at, h // G, None, None]).flatten(0, 1)[:L]
+            vv = (v[at, h // G] * vs[at, h // G, None, None]).flatten(0, 1)[:L]
+            s = q[cu[b]:cu[b + 1], h] @ kk.T * scale
+            s = s.masked_fill(torch.arange(L)[None] > torch.arange(L - n, L)[:, None], -float("inf"))
+            if sinks is not None:
+                s = torch.cat([s, sinks[h].double().cpu().expand(n, 1)], 1)
+            p = torch.softmax(s, 1)[:, :L]
+            out[cu[b]:cu[b + 1], h], mass[cu[b]:cu[b + 1], h] = p @ vv, p @ vv.abs()
+            unit[cu[b]:cu[b + 1], h] = (p @ vs[at, h // G].repeat_interleave(16)[:L])[:, None]
+    return out, mass, unit
+
+
+def far_check(got, want, mass, unit, keys):
+    """As ``check`` of the other file with each key's own scale: the output's rounding; a weight's (2^-11) and its
+    score's (2^-10), fp32 sums of 512 terms (2^-15), all of sum p |v|. The offset of 128 in the codes: terms of up to
+    255 p s added and taken out again, 2^-22 of each: 2^-13 sum p s. Products p s below f16's normal range are off by
+    up to 2^-25 where the largest of the row is at least 2^8, so by 2^-33 of it, times a code of up to 127: 2^-26 of
+    sum p s for each key."""
+    err = (got.cpu().double() - want).abs()
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -10 + 2.0 ** -15) * mass \
+        + (2.0 ** -13 + keys * 2.0 ** -26) * unit
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+def leaning(cache, tables, lens, exponents, d, hq, n, g, dev):
+    """V scales 2^e of the pages, and keys whose first column takes e log2 units off their scores, so that pages of all
+    scales count alike. ``exponents[b][p]`` = (e, units off)."""
+    for b in range(len(lens)):
+        for p, (e, off) in enumerate(exponents[b]):
+            at = tables[b, p].item()
+            cache[3][at] = 2.0 ** e
+            cache[2][at] = 2.0 ** -6
+            cache[0][at, :, :, 0] = max(-127, min(127, -off))
+    q = torch.randn(len(lens) * n, hq, d, generator=g) * 0.5
+    q[:, :, 0] = 64.0 * 0.6875 / d ** -0.5  # one code is 0.6875 * log2(e) = 0.992 log2 units
+    return q.to(dev, BF)
+
+
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("n", [1, 3])
+@pytest.mark.parametrize("hq,d", [(8, 128), (2, 128), (16, 64)])
+@pytest.mark.parametrize("kind", ["spread", "first", "middle", "last", "small first"])
+def test_v_scales_far_apart(cuda, kind, hq, d, n, sinks):
+    """A page whose scale is 2^60 times the others' and that has next to no weight, pages of all scales between 2^-40
+    and 2^40 that count alike, and a first page of tiny values."""
+    g = torch.Generator().manual_seed(hq + d + n)
+    lens = [33, 250, 3001]
+    tables, nb = make_tables(lens, g)
+    cache = make_cache(cuda, nb, 2, d, g)
+    exponents = []
+    for L in lens:
+        pages = (L + 15) // 16
+        if kind == "spread":
+            e = torch.randint(-40, 41, (pages,), generator=g).tolist()
+            exponents.append([(i, i) for i in e])
+        elif kind == "small first":
+            exponents.append([(-70, 0)] + [(-6, 0)] * (pages - 1))
+        else:
+            at = {"first": 0, "middle": pages // 2, "last": pages - 1}[kind]
+            exponents.append([(54, 110) if p == at else (-6, 0) for p in range(pages)])
+    q = leaning(cache, tables, lens, exponents, d, hq, n, g, cuda)
+    cu = [n * b for b in range(4)]
+    sk = torch.randn(hq, generator=g).to(cuda) if sinks else None
+    out = ops.paged_attention_int8(q, *cache, tables.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda),
+                                   cu_q=torch.tensor(cu, dtype=torch.int32, device=cuda), max_q_len=n,
+                                   scale=d ** -0.5, sinks=sk)
+    ops.check_errors(cuda)
+    want, mass, unit = far_oracle(q, cache, tables, lens, cu, d ** -0.5, sk)
+    far_check(out, want, mass, unit, max(lens))
