@@ -816,29 +816,33 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
               if (key > pos || (a.window > 0 && key <= pos - a.window) || j + p >= cnt) sc[p][nt][i] = -INFINITY;
             }
       }
-      // V scales in units, and the largest score of each row with their log2
+      // V scales in units and their log2. Scores of 2^24 and more are further apart than the limits: the distance to m
+      // is taken first, and m rounded up, so that no weight passes f16.
       float cv[PP], lv[PP];
 #pragma unroll
       for (int p = 0; p < PP; ++p) {
         cv[p] = fminf(sv[p] * per_unit, kFarScale);
         lv[p] = fmaxf(lg2(cv[p]), kNearLog);
       }
-      auto top = [&](int nt, int c) {
-        float mx = fmaxf(sc[0][nt][c], sc[0][nt][2 + c]) + lv[0];
-        if constexpr (PP == 2) mx = fmaxf(mx, fmaxf(sc[PP - 1][nt][c], sc[PP - 1][nt][2 + c]) + lv[PP - 1]);
-        return mx;
-      };
+      auto top = [&](int p, int nt, int c) { return fmaxf(sc[p][nt][c], sc[p][nt][2 + c]); };
       bool grow = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int p = 0; p < PP; ++p)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) grow |= top(nt, c) > m[nt][c] + kLimit;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) grow |= top(p, nt, c) - m[nt][c] > kLimit - lv[p];
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(m[nt][c], top(nt, c) - kShift);
+            float mx = m[nt][c];
+#pragma unroll
+            for (int p = 0; p < PP; ++p) {
+              const float t = top(p, nt, c);
+              mx = fmaxf(mx, fmaxf(t + (lv[p] - kShift), __fadd_ru(t, lv[p] - kLimit)));
+            }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));

@@ -110,3 +110,26 @@ def test_v_scales_far_apart(cuda, kind, hq, d, n, sinks):
     ops.check_errors(cuda)
     want, mass, unit = far_oracle(q, cache, tables, lens, cu, d ** -0.5, sk)
     far_check(out, want, mass, unit, max(lens))
+
+
+@pytest.mark.parametrize("power", [18, 20, 21, 24, 40])
+@pytest.mark.parametrize("n", [1, 4])
+def test_scores_beyond_the_spacing_of_fp32(cuda, power, n):
+    """Scores of 2^24 log2 units and more, whose neighbours in fp32 lie further apart than f16's exponents reach. One
+    column of q and of the keys is not zero, so scores are exact up to a factor common to the row: the largest keys of
+    each row share its weight."""
+    g = torch.Generator().manual_seed(power)
+    lens = [40, 333, 3000]
+    tables, nb = make_tables(lens, g)
+    cache = make_cache(cuda, nb, 2, 128, g)
+    cache[0][..., :5], cache[0][..., 6:] = 0, 0
+    cache[2].fill_(1.0)
+    q = torch.zeros(3 * n, 16, 128)
+    q[:, :, 5] = torch.randn(3 * n, 16, generator=g) * 2.0 ** power
+    q = q.to(cuda, BF)
+    cu = [n * b for b in range(4)]
+    out = ops.paged_attention_int8(q, *cache, tables.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda),
+                                   cu_q=torch.tensor(cu, dtype=torch.int32, device=cuda), max_q_len=n, scale=1.0)
+    ops.check_errors(cuda)
+    want, mass = oracle(q, cache, tables, lens, cu, 1.0)
+    check(out, want, mass, F16_EPS)
