@@ -20,6 +20,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -652,7 +653,8 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
       const int e = min(max((int)(am >> 7) - 127, -100), 100);
-      const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23);
+      // (the scale's sign goes with Q, so that factors are positive and one minimum bounds them)
+      const float down = copysignf(__int_as_float((127 - e) << 23), a.scale), up = __int_as_float((127 + e) << 23);
       float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
@@ -668,7 +670,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       sum *= -128.f / 16777216.f;
-      const float f = up * a.scale * (16777216.f * (a.softcap > 0.f ? 1.f : kLog2e));
+      const float f = fminf(up * fabsf(a.scale) * (16777216.f * (a.softcap > 0.f ? 1.f : kLog2e)), FLT_MAX);
       const int pos = pos0 + (row0 + nt * 8 + g) / a.G;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -788,7 +790,8 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) attn_kernel(const __gri
       for (int p = 0; p < PP; ++p)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float f0 = rs[nt][0] * sk[p], f1 = rs[nt][1] * sk[p];
+          // (finite for the largest K scales too: a product of zero stays zero)
+          const float f0 = fminf(rs[nt][0] * sk[p], FLT_MAX), f1 = fminf(rs[nt][1] * sk[p], FLT_MAX);
           sc[p][nt][0] *= f0;
           sc[p][nt][1] *= f1;
           sc[p][nt][2] *= f0;

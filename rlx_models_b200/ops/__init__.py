@@ -365,6 +365,9 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     ``max_q_len``), the last of its ``ctx_lens[b]`` tokens. ``sinks`` fp32 [Hq],
     ``window`` (0 = all) and ``softcap`` as in ``decode_attention``. A query that
     sees no key gives 0; rows of ``out`` behind cu_q[B] are left as they are.
+    A score is off by up to 2^-13 sum|q| s |scale|, s the block's K scale (sums of
+    terms of up to 255 |q| s in fp32); V scales of a sequence may lie up to 2^80
+    apart. Rows of ``q`` stay below 2^116.
     A call repeats its bits; equal sequences of one batch may differ in the last
     ones, for where a context is cut between warps depends on what lies before it.
 

@@ -133,3 +133,35 @@ def test_scores_beyond_the_spacing_of_fp32(cuda, power, n):
     ops.check_errors(cuda)
     want, mass = oracle(q, cache, tables, lens, cu, 1.0)
     check(out, want, mass, F16_EPS)
+
+
+@pytest.mark.parametrize("scale", [128 ** -0.5, -0.25])
+@pytest.mark.parametrize("n", [1, 3])
+def test_k_scales_near_the_largest(cuda, n, scale):
+    """Pages of K scale 2^120 whose products are zero (zero codes; codes only where q is zero) count as score 0, and
+    one whose product is not outweighs all others or nothing. q in eighths up to 2: sums of its products with codes
+    and with 128 are exact in fp32 (at most 128 * 255 * 2 = 2^16, in steps of 2^-3), as they have to be here: a
+    score is off by up to 2^-13 of sum |q| times the K scale."""
+    g = torch.Generator().manual_seed(n)
+    lens = [100, 3000, 48]
+    tables, nb = make_tables(lens, g)
+    cache = make_cache(cuda, nb, 2, 128, g)
+    for b, p in ((0, 2), (1, 0), (1, 100), (1, 187)):
+        at = tables[b, p].item()
+        cache[0][at] = 0
+        cache[0][at, :, :, 7] = 3
+        cache[2][at] = 2.0 ** 120
+    at = tables[2, 1].item()
+    cache[0][at] = 0
+    cache[0][at, :, 5, 9] = 1
+    cache[2][at] = 2.0 ** 120
+    q = (torch.randn(3 * n, 8, 128, generator=g) * 4).round().clamp(-16, 16) / 8
+    q[:, :, 7] = 0
+    q[:, :4, 9], q[:, 4:, 9] = 1.0, -1.0
+    q = q.to(cuda, BF)
+    cu = [n * b for b in range(4)]
+    out = ops.paged_attention_int8(q, *cache, tables.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda),
+                                   cu_q=torch.tensor(cu, dtype=torch.int32, device=cuda), max_q_len=n, scale=scale)
+    ops.check_errors(cuda)
+    want, mass = oracle(q, cache, tables, lens, cu, scale)
+    check(out, want, mass, F16_EPS)
