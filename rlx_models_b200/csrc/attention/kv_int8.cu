@@ -223,7 +223,9 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
   const int ctx = min(max(a.ctx_lens[b], 0), a.max_blocks * 16);
   if (p == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
     if (a.ctx_out != nullptr) a.ctx_out[b] = ctx;
-    if (a.ctx_lens[b] > ctx) report_error(a.status, kErrBounds, b);  // a context longer than its block table
+    // a context longer than its block table, more queries than max_q_len
+    if (a.ctx_lens[b] > ctx || (a.cu_q != nullptr && a.cu_q[b + 1] - a.cu_q[b] > a.max_q_len))
+      report_error(a.status, kErrBounds, b);
   }
   if (a.table_out != nullptr && blockIdx.y == 0 && threadIdx.x == 0) a.table_out[blockIdx.x] = blockIdx.x;
   const int pages = (ctx + 15) / 16, filled = (max(pages, 1) + a.pad - 1) / a.pad * a.pad;

@@ -691,11 +691,17 @@ static void check_int8_tables(const char* op, const Tensor& k_cache, const Tenso
 
 std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
                                           const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
-                                          Tensor& status, int64_t pad) {
+                                          Tensor& status, int64_t pad, const optional<Tensor>& cu_q,
+                                          int64_t max_q_len) {
   check_int8_cache("kv_dequant_pages_int8", k_cache, v_cache, k_scale, v_scale);
   check_int8_tables("kv_dequant_pages_int8", k_cache, block_tables, ctx_lens);
   const int64_t B = block_tables.size(0), mb = block_tables.size(1);
   TORCH_CHECK(pad >= 1 && pad <= 64, "b200.kv_dequant_pages_int8: 1 <= pad <= 64");
+  const bool queries = cu_q.has_value() && cu_q->defined();
+  if (queries)
+    TORCH_CHECK(cu_q->scalar_type() == at::kInt && cu_q->numel() == B + 1 && cu_q->is_contiguous() &&
+                    cu_q->device() == k_cache.device() && max_q_len >= 0 && max_q_len <= INT32_MAX,
+                "b200.kv_dequant_pages_int8: cu_q int32 [B + 1] on the caches' device");
   const int64_t ob = (mb + pad - 1) / pad * pad;  // blocks of a sequence in the copies
   TORCH_CHECK(B * ob <= INT32_MAX, "b200.kv_dequant_pages_int8: block_tables too large");
   c10::cuda::CUDAGuard g(k_cache.device());
@@ -716,6 +722,8 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   a.v_out = static_cast<__nv_bfloat16*>(v_out.data_ptr());
   a.table_out = table_out.data_ptr<int32_t>();
   a.ctx_out = bound ? ctx_out.data_ptr<int32_t>() : nullptr;
+  a.cu_q = queries ? cu_q->data_ptr<int32_t>() : nullptr;
+  a.max_q_len = (int)max_q_len;
   a.num_blocks = k_cache.size(0);
   a.B = (int)B;
   a.max_blocks = (int)mb;
@@ -1949,7 +1957,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_dequant_pages", &kv_dequant_pages);
   m.def("kv_store_int8", &kv_store_int8);
   m.def("kv_dequant_pages_int8", &kv_dequant_pages_int8, py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"),
-        py::arg("v_scale"), py::arg("block_tables"), py::arg("ctx_lens"), py::arg("status"), py::arg("pad") = 1);
+        py::arg("v_scale"), py::arg("block_tables"), py::arg("ctx_lens"), py::arg("status"), py::arg("pad") = 1,
+        py::arg("cu_q") = py::none(), py::arg("max_q_len") = 0);
   m.def("check_paged_attention_int8", &check_paged_attention_int8);
   m.def("paged_attention_int8", &paged_attention_int8);
   m.def("kv_copy_blocks", &kv_copy_blocks);

@@ -364,7 +364,9 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     [B + 1] sequence b has the queries cu_q[b] .. cu_q[b + 1] (at most
     ``max_q_len``), the last of its ``ctx_lens[b]`` tokens. ``sinks`` fp32 [Hq],
     ``window`` (0 = all) and ``softcap`` as in ``decode_attention``. A query that
-    sees no key gives 0; rows of ``out`` behind cu_q[B] are left as they are.
+    sees no key gives 0; rows of ``out`` behind cu_q[B] are left as they are. What
+    does not fit (a context longer than its block table, more queries than
+    ``max_q_len``) is left out and reported at the next ``check_errors``.
     A score is off by up to 2^-13 sum|q| s |scale|, s the block's K scale (sums of
     terms of up to 255 |q| s in fp32); V scales of a sequence may lie up to 2^80
     apart. Rows of ``q`` stay below 2^116.
@@ -395,7 +397,8 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         group = max(1, INT8_COPY_BYTES // (4 * (width + 7) * k_cache[0].numel()))
         for i in range(0, B, group):
             kb, vb, tables, ctx = ext().kv_dequant_pages_int8(
-                k_cache, v_cache, k_scale, v_scale, block_tables[i:i + group], ctx_lens[i:i + group], status, pad=8)
+                k_cache, v_cache, k_scale, v_scale, block_tables[i:i + group], ctx_lens[i:i + group], status, pad=8,
+                cu_q=cu_q[i:i + group + 1], max_q_len=int(max_q_len))
             _count(2)
             ext().prefill_attention(q, kb, vb, tables, ctx, cu_q[i:i + group + 1], out, sinks, int(window),
                                     float(scale), int(max_q_len), status, True, False, float(softcap), kv_contig=True)
