@@ -210,6 +210,11 @@ __device__ __forceinline__ uint2 widen_bf16(uint32_t w, float s) {
   return make_uint2(pack_bf16x2(f0, f1), pack_bf16x2(f2, f3));
 }
 
+// The queries lo .. hi of a sequence lie within q and are no more than announced.
+__device__ __forceinline__ bool queries_fit(int lo, int hi, int rows, int most) {
+  return lo >= 0 && lo <= hi && hi <= rows && hi - lo <= most;
+}
+
 // One CTA per (sequence, page, quarter of its heads' codes): 16 codes a thread
 // and step, up to four steps' loads in flight. 1 byte read and 2 written per
 // element: bound by HBM.
@@ -223,9 +228,14 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
   const int ctx = min(max(a.ctx_lens[b], 0), a.max_blocks * 16);
   if (p == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
     if (a.ctx_out != nullptr) a.ctx_out[b] = ctx;
-    // a context longer than its block table, more queries than max_q_len
-    if (a.ctx_lens[b] > ctx || (a.cu_q != nullptr && a.cu_q[b + 1] - a.cu_q[b] > a.max_q_len))
-      report_error(a.status, kErrBounds, b);
+    bool fits = a.ctx_lens[b] <= ctx;  // within its block table
+    if (a.cu_q != nullptr) {
+      const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
+      fits = fits && queries_fit(lo, hi, a.q_rows, a.max_q_len);
+      a.cu_out[b] = min(max(lo, 0), a.q_rows);  // attention over the copies stays within q
+      if (b == a.B - 1) a.cu_out[a.B] = min(max(hi, 0), a.q_rows);
+    }
+    if (!fits) report_error(a.status, kErrBounds, b);
   }
   if (a.table_out != nullptr && blockIdx.y == 0 && threadIdx.x == 0) a.table_out[blockIdx.x] = blockIdx.x;
   const int pages = (ctx + 15) / 16, filled = (max(pages, 1) + a.pad - 1) / a.pad * a.pad;
@@ -341,7 +351,7 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedInt8Args& a, int b) {
   if (a.cu_q != nullptr) {
     const int lo = a.cu_q[b], hi = a.cu_q[b + 1];
     s.q0 = min(max(lo, 0), a.T);
-    s.n = min(max(hi - lo, 0), min(a.T - s.q0, a.max_q_len));
+    s.n = hi > lo ? (int)min((int64_t)hi - lo, (int64_t)min(a.T - s.q0, a.max_q_len)) : 0;
   } else {
     s.q0 = b;
     s.n = 1;
@@ -367,10 +377,11 @@ __device__ __forceinline__ PageRange page_range(const PagedInt8Args& a, const Se
   return r;
 }
 
-// A context longer than its block table, or more queries than max_q_len: what does not fit is left out, and reported.
+// A context longer than its block table, queries that do not fit: what is too much is left out, and reported.
 __device__ __forceinline__ void check_seq(const PagedInt8Args& a, int b) {
-  const int n = a.cu_q != nullptr ? a.cu_q[b + 1] - a.cu_q[b] : 1;
-  if (a.ctx_lens[b] > (int64_t)a.max_blocks * 16 || n > a.max_q_len) report_error(a.status, kErrBounds, b);
+  if (a.ctx_lens[b] > (int64_t)a.max_blocks * 16 ||
+      (a.cu_q != nullptr && !queries_fit(a.cu_q[b], a.cu_q[b + 1], a.T, a.max_q_len)))
+    report_error(a.status, kErrBounds, b);
 }
 
 constexpr int kWholePages = 16;

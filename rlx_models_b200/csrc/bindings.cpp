@@ -692,7 +692,7 @@ static void check_int8_tables(const char* op, const Tensor& k_cache, const Tenso
 std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
                                           const Tensor& v_scale, const Tensor& block_tables, const Tensor& ctx_lens,
                                           Tensor& status, int64_t pad, const optional<Tensor>& cu_q,
-                                          int64_t max_q_len) {
+                                          int64_t max_q_len, int64_t q_rows) {
   check_int8_cache("kv_dequant_pages_int8", k_cache, v_cache, k_scale, v_scale);
   check_int8_tables("kv_dequant_pages_int8", k_cache, block_tables, ctx_lens);
   const int64_t B = block_tables.size(0), mb = block_tables.size(1);
@@ -700,7 +700,8 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   const bool queries = cu_q.has_value() && cu_q->defined();
   if (queries)
     TORCH_CHECK(cu_q->scalar_type() == at::kInt && cu_q->numel() == B + 1 && cu_q->is_contiguous() &&
-                    cu_q->device() == k_cache.device() && max_q_len >= 0 && max_q_len <= INT32_MAX,
+                    cu_q->device() == k_cache.device() && max_q_len >= 0 && max_q_len <= INT32_MAX && q_rows >= 0 &&
+                    q_rows <= INT32_MAX && mb > 0,
                 "b200.kv_dequant_pages_int8: cu_q int32 [B + 1] on the caches' device");
   const int64_t ob = (mb + pad - 1) / pad * pad;  // blocks of a sequence in the copies
   TORCH_CHECK(B * ob <= INT32_MAX, "b200.kv_dequant_pages_int8: block_tables too large");
@@ -711,6 +712,7 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   Tensor table_out = at::empty({B, ob}, block_tables.options());
   const bool bound = pad > 1 && ob > 0;  // for attention over the copies: ctx_lens within the table
   Tensor ctx_out = bound ? at::empty({B}, ctx_lens.options()) : ctx_lens;
+  Tensor cu_out = queries ? at::empty({B + 1}, cu_q->options()) : Tensor();
   b200::KvInt8DequantArgs a{};
   a.k_cache = k_cache.data_ptr<int8_t>();
   a.v_cache = v_cache.data_ptr<int8_t>();
@@ -724,6 +726,8 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   a.ctx_out = bound ? ctx_out.data_ptr<int32_t>() : nullptr;
   a.cu_q = queries ? cu_q->data_ptr<int32_t>() : nullptr;
   a.max_q_len = (int)max_q_len;
+  a.cu_out = queries ? cu_out.data_ptr<int32_t>() : nullptr;
+  a.q_rows = (int)q_rows;
   a.num_blocks = k_cache.size(0);
   a.B = (int)B;
   a.max_blocks = (int)mb;
@@ -734,6 +738,7 @@ std::vector<Tensor> kv_dequant_pages_int8(const Tensor& k_cache, const Tensor& v
   a.status = status.data_ptr<int>();
   b200::kv_int8_dequant_launch(a, cur_stream(k_cache));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (queries) return {k_out, v_out, table_out, ctx_out, cu_out};
   return {k_out, v_out, table_out, ctx_out};
 }
 
@@ -1958,7 +1963,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_store_int8", &kv_store_int8);
   m.def("kv_dequant_pages_int8", &kv_dequant_pages_int8, py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"),
         py::arg("v_scale"), py::arg("block_tables"), py::arg("ctx_lens"), py::arg("status"), py::arg("pad") = 1,
-        py::arg("cu_q") = py::none(), py::arg("max_q_len") = 0);
+        py::arg("cu_q") = py::none(), py::arg("max_q_len") = 0, py::arg("q_rows") = 0);
   m.def("check_paged_attention_int8", &check_paged_attention_int8);
   m.def("paged_attention_int8", &paged_attention_int8);
   m.def("kv_copy_blocks", &kv_copy_blocks);

@@ -364,8 +364,9 @@ struct KvInt8DequantArgs {
   __nv_bfloat16* k_out;
   __nv_bfloat16* v_out;
   int32_t* ctx_out;         // [B] or null: ctx_lens within [0, 16 max_blocks]
-  const int32_t* cu_q;      // [B + 1] or null: query offsets; more than max_q_len of a sequence are reported
-  int max_q_len;
+  const int32_t* cu_q;      // [B + 1] or null: query offsets; more than max_q_len of a sequence, and offsets outside
+  int32_t* cu_out;          // [0, q_rows], are reported; [B + 1]: the offsets within
+  int max_q_len, q_rows;
   int32_t* table_out;       // [B, out_blocks] or null: the copies' block table, 0, 1, 2 ...
   int64_t num_blocks;
   int B, max_blocks, Hkv, D;

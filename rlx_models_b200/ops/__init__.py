@@ -366,7 +366,7 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     ``window`` (0 = all) and ``softcap`` as in ``decode_attention``. A query that
     sees no key gives 0; rows of ``out`` behind cu_q[B] are left as they are. What
     does not fit (a context longer than its block table, more queries than
-    ``max_q_len``) is left out and reported at the next ``check_errors``.
+    ``max_q_len``, offsets outside ``q``) is left out and reported at the next ``check_errors``.
     A score is off by up to 2^-13 sum|q| s |scale|, s the block's K scale (sums of
     terms of up to 255 |q| s in fp32); V scales of a sequence may lie up to 2^80
     apart. Rows of ``q`` stay below 2^116.
@@ -396,11 +396,11 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         B, width = block_tables.shape
         group = max(1, INT8_COPY_BYTES // (4 * (width + 7) * k_cache[0].numel()))
         for i in range(0, B, group):
-            kb, vb, tables, ctx = ext().kv_dequant_pages_int8(
+            kb, vb, tables, ctx, cu = ext().kv_dequant_pages_int8(
                 k_cache, v_cache, k_scale, v_scale, block_tables[i:i + group], ctx_lens[i:i + group], status, pad=8,
-                cu_q=cu_q[i:i + group + 1], max_q_len=int(max_q_len))
+                cu_q=cu_q[i:i + group + 1], max_q_len=int(max_q_len), q_rows=q.shape[0])
             _count(2)
-            ext().prefill_attention(q, kb, vb, tables, ctx, cu_q[i:i + group + 1], out, sinks, int(window),
+            ext().prefill_attention(q, kb, vb, tables, ctx, cu, out, sinks, int(window),
                                     float(scale), int(max_q_len), status, True, False, float(softcap), kv_contig=True)
         return out
     out, n = ext().paged_attention_int8(q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens, cu_q,
