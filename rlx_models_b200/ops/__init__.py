@@ -373,6 +373,9 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     A call repeats its bits; equal sequences of one batch may differ in the last
     ones, for where a context is cut between warps depends on what lies before it.
 
+    ``block_tables`` should be no wider than the longest context needs: copies (below)
+    and the grid follow its width, since lengths are known on the device only.
+
     Up to ``INT8_DIRECT_ROWS`` query rows per KV head the pages are read as they
     are. Longer chunks are bound by their products and go through bf16 copies of
     the pages to the tcgen05 kernel of ``prefill_attention`` where it applies
@@ -387,7 +390,8 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
             and q.shape[1] in [g * k_cache.shape[1] for g in (1, 2, 4, 8)] and softcap <= 0
             and block_tables.shape[-1] > 0):
         # copies of a sequence lie in a row and end on a multiple of 8 pages: one box of the kernel's loads. The table's
-        # width decides how much memory they take: so many sequences at a time that it stays within INT8_COPY_BYTES
+        # width decides how much memory they take: so many sequences at a time that it stays within INT8_COPY_BYTES,
+        # or one whose copies alone take more
         status = scratch(q.device).status
         if out is None:
             out = torch.empty_like(q)
@@ -396,6 +400,7 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         B, width = block_tables.shape
         group = max(1, INT8_COPY_BYTES // (4 * (width + 7) * k_cache[0].numel()))
         for i in range(0, B, group):
+            kb = vb = None  # given back before the next ones are made
             kb, vb, tables, ctx, cu = ext().kv_dequant_pages_int8(
                 k_cache, v_cache, k_scale, v_scale, block_tables[i:i + group], ctx_lens[i:i + group], status, pad=8,
                 cu_q=cu_q[i:i + group + 1], max_q_len=int(max_q_len), q_rows=q.shape[0])

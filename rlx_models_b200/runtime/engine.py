@@ -430,10 +430,15 @@ class LLMEngine:
                            seq_slots=nd + npf if self.stateful else 0, tok_src=nd))
         if nd:  # decode inputs still being sampled by the previous step
             ops.forward_tokens(d["input_ids"][:nd], d["tok_src"][:nd], self.tok_out)
+        pre_tables = d["pre_tables"][:npf] if npf else None
+        if npf and getattr(self.kv, "k_scale", None) is not None:
+            # int8: the bf16 copies of a chunk's pages are as many as its table is wide
+            longest = int(self.h["pre_ctx"][:npf].max())
+            pre_tables = pre_tables[:, :(longest + BLOCK_SIZE - 1) // BLOCK_SIZE].contiguous()
         fb = ForwardBatch(
             input_ids=d["input_ids"][:T], positions=d["positions"][:T], slots=d["slots"][:T], num_decode=nd,
             dec_block_tables=d["dec_tables"][:nd] if nd else None, dec_ctx_lens=d["dec_ctx"][:nd] if nd else None,
-            pre_block_tables=d["pre_tables"][:npf] if npf else None,
+            pre_block_tables=pre_tables,
             pre_ctx_lens=d["pre_ctx"][:npf] if npf else None, pre_cu_q=d["pre_cu"][:npf + 1] if npf else None,
             pre_max_q=max_q, logit_rows=d["logit_rows"][:R],
             seq_slots=d["seq_slots"][:nd + npf] if self.stateful else None,

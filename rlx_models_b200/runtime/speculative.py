@@ -83,10 +83,11 @@ class _Seq:
         ctx = start + n
         if ctx > self.nb * 16:
             raise ValueError("sequence longer than the speculative decoder's max_len")
+        table = self.table[:, :(ctx + 15) // 16] if self.int8 else self.table  # (as wide as the copies of its pages)
         fb = ForwardBatch(input_ids=torch.tensor(tokens, dtype=torch.int32, device=dev),
                           positions=torch.arange(start, ctx, dtype=torch.int32, device=dev),
                           slots=torch.arange(start, ctx, dtype=torch.int64, device=dev), num_decode=0,
-                          pre_block_tables=self.table, pre_ctx_lens=torch.tensor([ctx], dtype=torch.int32, device=dev),
+                          pre_block_tables=table, pre_ctx_lens=torch.tensor([ctx], dtype=torch.int32, device=dev),
                           pre_cu_q=torch.tensor([0, n], dtype=torch.int32, device=dev), pre_max_q=n)
         if keep_hidden:
             h = self.model.forward_hidden(fb, self.kv)
