@@ -45,7 +45,31 @@ constexpr int kStoreWarps = 4;
 // and stores, 32-byte bf16 loads, all rows of the block in flight at once. The
 // kernel moves 3 bytes per element and is bound by launch and load latency for
 // a decode step, by HBM for a prefill.
-template <int D>
+//
+// Two runs of one block would be two warps that write one block and its scale, so
+// only one of them does and the other is reported. In batches of up to kScan tokens
+// a warp looks at the slots before its run, asked for beside its own; longer ones
+// have a launch in front in which every run writes its name to its block's owner
+// (whichever comes last stays), with nothing to clear first. 64 tokens of 64
+// requests 3.0 us without the look and 3.2 with it, 256 5.3 and 5.9; a prompt of 1000
+// 6.9 and 7.8 with the launch, of 8192 10.7 and 12.1 (8 heads of 128).
+constexpr int kScan = 256;
+
+// The first token of a run: a slot whose block is not the one before it.
+__device__ __forceinline__ bool run_begins(int64_t before, int64_t slot) {
+  return slot >= 0 && (before < 0 || (before >> 4) != (slot >> 4));
+}
+
+__global__ void __launch_bounds__(256) owner_kernel(KvInt8StoreArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= a.T) return;
+  const int64_t slot = a.slots[t], before = t > 0 ? a.slots[t - 1] : -1;
+  if (run_begins(before, slot) && (slot >> 4) < a.num_blocks) a.owner[slot >> 4] = (int32_t)t;
+}
+
+template <int D, bool kOwner>
 __global__ void __launch_bounds__(kStoreWarps * 32, 6) store_kernel(KvInt8StoreArgs a) {
   pdl_wait();
   pdl_trigger();
@@ -70,8 +94,14 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 6) store_kernel(KvInt8StoreA
   const int64_t near = t0 + lane < a.T ? a.slots[t0 + lane] : -1;
   int64_t ahead = __shfl_up_sync(0xffffffffu, near, 1);
   if (lane == 0) ahead = t0 > 0 ? a.slots[t0 - 1] : -1;
-  unsigned firsts =
-      __ballot_sync(0xffffffffu, t0 + lane < t1 && near >= 0 && (ahead < 0 || (ahead >> 4) != (near >> 4)));
+  constexpr int kPrior = kOwner ? 0 : kScan / 32;
+  uint32_t prior[kPrior + 1];  // low words of the slots in front (lane i: tokens i, 32 + i ...)
+#pragma unroll
+  for (int i = 0; i < kPrior; ++i) {
+    const int t = i * 32 + lane;
+    prior[i] = t < t0 ? reinterpret_cast<const uint32_t*>(a.slots)[2 * t] : ~0u;
+  }
+  unsigned firsts = __ballot_sync(0xffffffffu, t0 + lane < t1 && run_begins(ahead, near));
   while (firsts != 0) {
     const int at = __ffs(firsts) - 1;
     firsts &= firsts - 1;
@@ -82,6 +112,15 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 6) store_kernel(KvInt8StoreA
     }
     const int64_t page = blk * a.Hkv + h;
     const float old = scales[page];  // (asked for early; used when the block is not new)
+    bool other = false;  // a run of this block elsewhere in the batch
+    if constexpr (kOwner) other = a.owner[blk] != (int32_t)(t0 + at);
+#pragma unroll
+    for (int i = 0; i < kPrior; ++i)
+      if ((prior[i] >> 4) == (uint32_t)blk) other |= (a.slots[i * 32 + lane] >> 4) == blk;
+    if (__any_sync(0xffffffffu, other)) {
+      if (lane == 0) report_error(a.status, kErrOrder, (int)min(blk, (int64_t)0x7fffffff));
+      continue;
+    }
     // lane o < 16: newest token of the run written at offset o, from t0 (-1: none)
     int src = -1;
     int64_t slot = __shfl_down_sync(0xffffffffu, near, at);
@@ -1072,19 +1111,25 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(PagedInt8Args a, i
 
 }  // namespace kv8
 
-void kv_int8_store_launch(const KvInt8StoreArgs& args, int D, cudaStream_t st) {
+int64_t kv_int8_store_scan() { return kv8::kScan; }
+
+int kv_int8_store_launch(const KvInt8StoreArgs& args, int D, cudaStream_t st) {
   using namespace kv8;
-  if (args.T == 0 || args.Hkv == 0) return;
+  if (args.T == 0 || args.Hkv == 0) return 0;
   KvInt8StoreArgs a = args;
   // one token per warp keeps every warp on its own block when blocks get one token each (a decode
   // step); longer batches are prefill, where 15 of 16 warps would find that they have nothing to do
   a.group = a.T <= 1024 ? 1 : 16;
   const int64_t tasks = (a.T + a.group - 1) / a.group * a.Hkv * 2;
   const unsigned grid = (unsigned)((tasks + kStoreWarps - 1) / kStoreWarps);
-  if (D == 128)
-    launch_pdl(store_kernel<128>, dim3(grid), dim3(kStoreWarps * 32), 0, st, a);
-  else
-    launch_pdl(store_kernel<64>, dim3(grid), dim3(kStoreWarps * 32), 0, st, a);
+  auto run = [&](auto kernel) { launch_pdl(kernel, dim3(grid), dim3(kStoreWarps * 32), 0, st, a); };
+  if (a.owner != nullptr) {
+    launch_pdl(owner_kernel, dim3((unsigned)((a.T + 255) / 256)), dim3(256), 0, st, a);
+    D == 128 ? run(store_kernel<128, true>) : run(store_kernel<64, true>);
+  } else {
+    D == 128 ? run(store_kernel<128, false>) : run(store_kernel<64, false>);
+  }
+  return a.owner != nullptr ? 2 : 1;
 }
 
 void kv_int8_dequant_launch(const KvInt8DequantArgs& a, cudaStream_t st) {

@@ -645,8 +645,8 @@ static Tensor aligned_rows(const Tensor& t) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
-void kv_store_int8(const Tensor& k_in, const Tensor& v_in, const Tensor& slots, Tensor& k_cache, Tensor& v_cache,
-                   Tensor& k_scale, Tensor& v_scale, Tensor& status) {
+int64_t kv_store_int8(const Tensor& k_in, const Tensor& v_in, const Tensor& slots, Tensor& k_cache, Tensor& v_cache,
+                      Tensor& k_scale, Tensor& v_scale, Tensor& status) {
   check_int8_cache("kv_store_int8", k_cache, v_cache, k_scale, v_scale);
   c10::cuda::CUDAGuard g(k_cache.device());
   const Tensor k = aligned_rows(k_in), v = aligned_rows(v_in);
@@ -676,8 +676,15 @@ void kv_store_int8(const Tensor& k_in, const Tensor& v_in, const Tensor& slots, 
   a.num_blocks = k_cache.size(0);
   a.Hkv = (int)Hkv;
   a.status = status.data_ptr<int>();
-  b200::kv_int8_store_launch(a, (int)D, cur_stream(k_cache));
+  TORCH_CHECK(T <= INT32_MAX, "b200.kv_store_int8: too many tokens");
+  Tensor owner;  // of this call; blocks that it does not touch keep whatever is there
+  if (T > b200::kv_int8_store_scan()) {
+    owner = at::empty({k_cache.size(0)}, slots.options().dtype(at::kInt));
+    a.owner = owner.data_ptr<int32_t>();
+  }
+  const int n = b200::kv_int8_store_launch(a, (int)D, cur_stream(k_cache));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return n;
 }
 
 static void check_int8_tables(const char* op, const Tensor& k_cache, const Tensor& tables, const Tensor& ctx) {

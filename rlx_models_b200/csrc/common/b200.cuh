@@ -38,6 +38,7 @@ enum ErrCode : int {
   kErrBounds = 7,           // debug bounds check failed
   kErrTimeoutDrain = 8,     // draining in-flight copies on the error path
   kErrTimeoutTest = 9,      // deliberate timeout used by tests (flag never set)
+  kErrOrder = 10,           // rows of one KV block apart in the batch
 };
 
 constexpr unsigned long long kWaitTimeoutNs = 2000000000ull;  // 2 s

@@ -348,10 +348,12 @@ struct KvInt8StoreArgs {
   float* v_scale;
   int64_t T, num_blocks;
   int Hkv;
+  int32_t* owner = nullptr;  // [num_blocks], more than kv_int8_store_scan() tokens: the run that writes a block
   int group = 1;           // tokens per warp (set by the launcher)
   int* status;
 };
-void kv_int8_store_launch(const KvInt8StoreArgs& a, int D, cudaStream_t st);
+int64_t kv_int8_store_scan();  // tokens up to which warps look for other runs themselves
+int kv_int8_store_launch(const KvInt8StoreArgs& a, int D, cudaStream_t st);  // returns #launches
 
 // bf16 copies of the pages of a prefill batch at block b * max_blocks + p (as kv_dequant_pages_launch)
 struct KvInt8DequantArgs {

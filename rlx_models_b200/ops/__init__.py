@@ -332,9 +332,10 @@ def kv_store_int8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache
     counts in the maximum.
 
     The tokens of one block must be adjacent in the batch, without skipped rows
-    between them; a slot that comes twice among them takes the later row."""
-    _count(1)
-    ext().kv_store_int8(k, v, slots, k_cache, v_cache, k_scale, v_scale, scratch(k_cache.device).status)
+    between them; a slot that comes twice among them takes the later row. Of several
+    such runs of one block only one is stored (the first in batches of up to 256
+    tokens), and an error reported at the next ``check_errors``."""
+    _count(ext().kv_store_int8(k, v, slots, k_cache, v_cache, k_scale, v_scale, scratch(k_cache.device).status))
 
 
 def kv_dequant_pages_int8(k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens):

@@ -72,7 +72,7 @@ class KernelError(RuntimeError):
         1: "TMA stage wait timed out", 2: "free-stage wait timed out",
         3: "accumulator wait timed out", 4: "accumulator release wait timed out",
         5: "peer flag wait timed out", 6: "split-K wait timed out", 7: "bounds check failed",
-        8: "drain wait timed out", 9: "test timeout",
+        8: "drain wait timed out", 9: "test timeout", 10: "rows of one KV block are not adjacent in the batch",
     }
 
     def __init__(self, st):
