@@ -865,6 +865,17 @@ void kv_copy_blocks(const std::vector<Tensor>& src, const std::vector<Tensor>& d
     p.src_layer = bytes * a.src_blocks;
     p.dst_layer = bytes * a.dst_blocks;
   }
+  // copies run in no order: what one part writes no other part reads or writes, nor the same one at another place
+  auto meet = [](const Tensor& x, const Tensor& y) {
+    const auto *p = static_cast<const uint8_t*>(x.data_ptr()), *q = static_cast<const uint8_t*>(y.data_ptr());
+    return x.numel() > 0 && y.numel() > 0 && p < q + y.nbytes() && q < p + x.nbytes();
+  };
+  for (size_t j = 0; j < dst.size(); ++j)
+    for (size_t i = 0; i < src.size(); ++i)
+      TORCH_CHECK((!meet(src[i], dst[j]) || (i == j && src[i].data_ptr() == dst[j].data_ptr() &&
+                                             (a.src_blocks == a.dst_blocks || a.layers == 1))) &&
+                      (i >= j || !meet(dst[i], dst[j])),
+                  "b200.kv_copy_blocks: a destination overlaps another tensor of the call");
   c10::cuda::CUDAGuard g(dev);
   a.src_ids = src_ids.data_ptr<int32_t>();
   a.dst_ids = dst_ids.data_ptr<int32_t>();

@@ -425,7 +425,7 @@ def _block_ids(ids, device) -> torch.Tensor:
 def kv_copy_blocks(src, dst, src_ids, dst_ids) -> None:
     """``dst[i][:, dst_ids] = src[i][:, src_ids]`` for up to four tensors
     [layers, blocks, ...] of a cache (K, V, scales), all layers in one launch.
-    ``src`` and ``dst`` may be the same tensors. Block ids: int32 tensors [n] on
+    ``src`` and ``dst`` may be the same tensors, but not overlap otherwise. Block ids: int32 tensors [n] on
     the device (negative: skip), or lists, which are checked here. A block may be
     copied to several places; the places must differ, and none may be a source
     of the same call (copies run in no order)."""
@@ -438,7 +438,7 @@ def kv_copy_blocks(src, dst, src_ids, dst_ids) -> None:
             raise ValueError("kv_copy_blocks: block id out of range")
         if len(set(dst_ids)) != len(dst_ids):
             raise ValueError("kv_copy_blocks: a destination block comes twice")
-        if src[0].data_ptr() == dst[0].data_ptr() and set(src_ids) & set(dst_ids):
+        if any(s.data_ptr() == d.data_ptr() for s, d in zip(src, dst) if s.numel()) and set(src_ids) & set(dst_ids):
             raise ValueError("kv_copy_blocks: a destination block is also a source")
     dev = src[0].device
     _count(1)
