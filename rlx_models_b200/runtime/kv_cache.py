@@ -87,7 +87,7 @@ class PagedKVCache:
         dst = self.tensors()
         if set(saved) != set(dst):
             raise ValueError(f"KV blocks hold {sorted(saved)}, this cache {sorted(dst)}")
-        if src:
+        if len(src):
             ops.kv_copy_blocks([saved[n].to(t.device) for n, t in dst.items()], list(dst.values()), src, blocks)
 
     @staticmethod

@@ -26,6 +26,7 @@ from ..weights.safetensors_io import SafetensorsFile, save_file
 from .kv_cache import BLOCK_SIZE
 
 FORMAT = "rlx_models_b200.prompt_cache/1"
+COPY_BYTES = 256 << 20  # of device memory beside the cache for blocks on their way
 
 
 def model_fingerprint(model, kv) -> str:
@@ -49,6 +50,10 @@ def model_fingerprint(model, kv) -> str:
     return h.hexdigest()
 
 
+def _blocks_at_once(kv) -> int:
+    return max(1, COPY_BYTES // sum(t[:, :1].numel() * t.element_size() for t in kv.tensors().values()))
+
+
 def save_prompt(engine, path: str, tokens: list[int]) -> int:
     """Write the cached KV of ``tokens``' longest cached full-block prefix;
     returns the number of tokens saved (0: nothing cached)."""
@@ -57,7 +62,11 @@ def save_prompt(engine, path: str, tokens: list[int]) -> int:
     n = len(blocks)
     kv = engine.kv
     if n:
-        tensors = {name: t.cpu() for name, t in kv.gather_blocks(blocks).items()}
+        tensors = {name: torch.empty((t.shape[0], n) + t.shape[2:], dtype=t.dtype) for name, t in kv.tensors().items()}
+        step = _blocks_at_once(kv)
+        for i in range(0, n, step):
+            for name, t in kv.gather_blocks(blocks[i:i + step]).items():
+                tensors[name][:, i:i + step].copy_(t)
     else:
         tensors = {"k": torch.empty(0), "v": torch.empty(0)}
     tensors["tokens"] = torch.tensor(tokens[:n * BLOCK_SIZE], dtype=torch.int32)
@@ -82,8 +91,13 @@ def load_prompt(engine, path: str) -> int:
         kv = engine.kv
         fill = [(i, b) for i, b in enumerate(blocks) if b >= 0]
         if fill:
-            saved = {name: f.get(name).clone() for name in kv.tensors()}  # copies: the file's mapping closes below
-            kv.scatter_blocks(saved, [i for i, _ in fill], [b for _, b in fill])
+            step = _blocks_at_once(kv)
+            for at in range(0, len(fill), step):
+                some = fill[at:at + step]
+                src = torch.tensor([i for i, _ in some])
+                # (copies: no view of the file's mapping may be left when it closes)
+                kv.scatter_blocks({name: f.get(name).index_select(1, src) for name in kv.tensors()}, range(len(some)),
+                                  [b for _, b in some])
         return len(blocks) * BLOCK_SIZE
     finally:
         f.close()
