@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kDequantThreads) dequant_kernel(KvInt8DequantA
 // Where the host knows that no segment has more than kWholePages pages (a sliding
 // window, a narrow block table), warps take whole segments in turn instead: no
 // prefix sums, no parts, no second launch (128 requests with a window of 128
-// tokens: 10.9 us instead of 20.0).
+// tokens: 11.2 us instead of 20).
 //
 // Each warp has its own TMA ring, running maximum, sum and accumulators. Both
 // products run transposed, S^T = K Q^T and O^T = V^T P^T (mma m16n8k16, f16

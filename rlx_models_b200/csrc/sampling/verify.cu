@@ -9,8 +9,10 @@
 //   T <= 0: accept while d_i is the (lowest) argmax, then take the argmax.
 //
 // Decisions are whole numbers, so what decides them is held in 64 bits: with
-// 1.5e5 tokens the borders of the running sum lie 1e-5 apart and closer, and sums
-// of 32-bit exponentials would move one draw in a thousand across a border.
+// 1.5e5 tokens the borders of the drawn row's running sum lie 1e-5 apart and closer,
+// and sums of 32-bit exponentials would move one draw in a thousand across a border;
+// an acceptance needs them where u q lies next to p. Which rows are drawn or close is
+// known after the statistics only, so all rows have them in 64 bits.
 // An exponential (Exp64) takes 8 double-precision operations, so 34 M logits (64
 // requests of 3.5 rows of 151936) are 15 us of the double-precision pipes under
 // the 21 us that their 136 MB take from HBM.

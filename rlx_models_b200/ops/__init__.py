@@ -380,7 +380,9 @@ def paged_attention_int8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     Up to ``INT8_DIRECT_ROWS`` query rows per KV head the pages are read as they
     are. Longer chunks are bound by their products and go through bf16 copies of
     the pages to the tcgen05 kernel of ``prefill_attention`` where it applies
-    (D 128, groups of 1, 2, 4 or 8, no softcap). Measured on a B200 with 8 KV
+    (D 128, groups of 1, 2, 4 or 8, no softcap). Weights are rounded to f16 in the
+    first way and to bf16 in the second (error against 64 bits 0.0017 and 0.0023 of
+    the output). Measured on a B200 with 8 KV
     heads, direct / by copies: 64 sequences of 1400 tokens, 64 rows 146 / 179 us,
     80 rows 212 / 179 us; 16 of 2400 tokens 74 / 72 and 97 / 72 us. That kernel
     does not split a context: few sequences are better off directly for longer (2

@@ -109,7 +109,8 @@ class EngineConfig:
     kv_retrieval: dict | None = None
     # "bf16"; "fp8": float8 e4m3 pages holding value / scale with scales (k, v) (the
     # decode kernel reads them directly; prefill reads bf16 copies of its pages); "int8":
-    # codes with a scale for each block and KV head, no scales to choose
+    # codes with a scale for each block and KV head, no scales to choose (prompt chunks take
+    # bf16 copies of their pages, up to 1 GiB beside kv_memory_gb)
     kv_cache_dtype: str = "bf16"
     kv_cache_scales: tuple = (1.0, 1.0)
     # schedule / launch step n+1 before step n's tokens come back (see module docstring)
