@@ -535,8 +535,8 @@ bool fmha_supported(const AttnArgs& a) {
     return e != nullptr && e[0] == '1';
   }();
   const int G = a.Hq / a.Hkv;
-  // logit softcapping runs on the mma.sync kernel
-  return !legacy && a.D == 128 && a.softcap <= 0.f && a.Hq % a.Hkv == 0 && G >= 1 && G <= 8 &&
+  // logit softcapping runs on the mma.sync kernel, and so do scales below 0: row maxima are taken before the scale here
+  return !legacy && a.D == 128 && a.softcap <= 0.f && a.scale >= 0.f && a.Hq % a.Hkv == 0 && G >= 1 && G <= 8 &&
          (G & (G - 1)) == 0 && a.q_rows > 0;
 }
 
