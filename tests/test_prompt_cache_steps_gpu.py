@@ -34,9 +34,9 @@ def test_roundtrip_in_steps(cuda, tmp_path, monkeypatch, dtype, blocks):
     def peak(f, *args):
         torch.cuda.synchronize()
         torch.cuda.reset_peak_memory_stats()
-        before = torch.cuda.memory_allocated()
+        before = torch.cuda.memory_stats()["requested_bytes.all.current"]
         assert f(*args) == 192
-        return torch.cuda.max_memory_allocated() - before
+        return torch.cuda.memory_stats()["requested_bytes.all.peak"] - before
 
     e1.save_prompt_cache(path, prompt)
     e2.generate([prompt[:70] + [3, 1, 4]], sp)  # four of the twelve blocks are there already
